@@ -174,6 +174,16 @@ PROTOTYPES = {
                              ctypes.POINTER(KvAppendEpilogue), _vp]),
     "spa_decoder_step_workspace_size": (_sz, [ctypes.POINTER(DecoderStepParams)]),
     "spa_decoder_step": (_i, [ctypes.POINTER(DecoderStepParams), _vp]),
+    "spa_int4_append": (_i, [_KV, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "spa_int4_read": (_i, [_KV, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
+    "spa_cache_decode_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "spa_int4_decode": (_i, [_vp, _i, _i, _i, _i, _i, _KV, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _d, _vp, _vp, _i, _vp,
+                             _sz, _vp]),
+    "spa_paged_decode_weights": (_i, [_vp, _i, _i, _i, _i, _i, _KV, _vp, _i, _i, _i, _d, _vp, _vp, _i, _vp, _sz,
+                                      _vp]),
+    "spa_select_tokens": (_i, [_vp, _i, _i, _i, _vp, _i, _i, _vp, _vp, _vp]),
+    "spa_compact_tokens": (_i, [_KV, _i, ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(_i), _i, _i, _vp, _i, _vp,
+                                _i, _vp]),
 }
 
 

@@ -3,6 +3,8 @@ per-device cached buffers (workspaces, constant length vectors)."""
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import _lib
@@ -23,6 +25,14 @@ def stream_ptr(device: torch.device | int) -> int:
     if index is None:
         index = torch.cuda.current_device()
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Makes ``device`` the current one for a launch (free when it already is)."""
+    return _SAME_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def require_cuda(*tensors: torch.Tensor, message: str = "CUDA tensors are required") -> None:

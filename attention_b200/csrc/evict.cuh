@@ -1,0 +1,257 @@
+// Eviction from a paged cache by accumulated attention weight: which tokens stay
+// (select_tokens_kernel), and their move to the front of the sequence (compact_kernel).
+#pragma once
+
+#include "common.cuh"
+
+namespace spa {
+
+// Order-preserving map of a weight: larger key = larger weight, -0 = +0, NaN below all.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  uint32_t u = __float_as_uint(w);
+  if (u == 0x80000000u) u = 0u;
+  if (w != w) return 0u;
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+// One CTA per (kv head, sequence).  The last r tokens stay; of the n = L - r before them the
+// `need` largest keys, ties to the lower token.  The need-th largest key is found digit by
+// digit (11, 11 and 10 bits, a histogram each), then one pass in token order writes the
+// tokens above it and the first of those equal to it.
+constexpr int kSelThreads = 1024;
+
+__global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(const float* __restrict__ weights, int T,
+                                                                    const int32_t* __restrict__ lens, int budget,
+                                                                    int recent, int32_t* __restrict__ keep,
+                                                                    int32_t* __restrict__ kept_lens) {
+  __shared__ int hist[2048];
+  __shared__ int wsum[kSelThreads / 32][2];
+  __shared__ uint32_t s_prefix;
+  __shared__ int s_need;
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t bh = static_cast<int64_t>(b) * gridDim.x + h;
+  const float* w = weights + bh * T;
+  int32_t* out = keep + bh * budget;
+  const int L = min(max(lens[b], 0), T);
+  if (h == 0 && tid == 0) kept_lens[b] = min(L, budget);
+  if (L <= budget) {
+    for (int i = tid; i < budget; i += kSelThreads) out[i] = i < L ? i : -1;
+    return;
+  }
+  const int r = min(recent, budget), n = L - r, need0 = budget - r;
+  for (int i = tid; i < r; i += kSelThreads) out[need0 + i] = n + i;
+  if (need0 == 0) return;
+  uint32_t prefix = 0, mask = 0;
+  int need = need0;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kSelThreads) {
+      const uint32_t k = weight_key(w[i]);
+      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1);
+    }
+    __syncthreads();
+    if (warp == 0) {
+      // from the top bin down, 64 bins per lane, until `need` keys are covered
+      const int per = (1 << bits) / 32, top = (1 << bits) - 1 - lane * per;
+      int sum = 0;
+      for (int i = 0; i < per; ++i) sum += hist[top - i];
+      int inc = sum;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, inc, off);
+        if (lane >= off) inc += o;
+      }
+      int before = inc - sum;
+      if (before < need && inc >= need) {
+        int i = 0;
+        while (before + hist[top - i] < need) before += hist[top - i++];
+        s_prefix = prefix | (static_cast<uint32_t>(top - i) << shift);
+        s_need = need - before;
+      }
+    }
+    __syncthreads();
+    prefix = s_prefix;
+    need = s_need;
+    mask |= ((1u << bits) - 1) << shift;
+  }
+  // tokens above the threshold and the first `need` equal to it, in token order
+  int above0 = 0, equal0 = 0;
+  for (int base = 0; base < n; base += kSelThreads) {
+    const int i = base + tid;
+    const uint32_t k = i < n ? weight_key(w[i]) : 0u;
+    const bool gt = i < n && k > prefix, eq = i < n && k == prefix;
+    const unsigned bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
+    if (lane == 0) {
+      wsum[warp][0] = __popc(bg);
+      wsum[warp][1] = __popc(be);
+    }
+    __syncthreads();
+    int above = above0, equal = equal0, ta = 0, te = 0;
+    for (int v = 0; v < kSelThreads / 32; ++v) {
+      if (v < warp) above += wsum[v][0], equal += wsum[v][1];
+      ta += wsum[v][0];
+      te += wsum[v][1];
+    }
+    const unsigned lt = (1u << lane) - 1;
+    above += __popc(bg & lt);
+    equal += __popc(be & lt);
+    if (gt || (eq && equal < need)) out[above + min(equal, need)] = i;
+    above0 += ta;
+    equal0 += te;
+    __syncthreads();
+  }
+}
+
+// In-place compaction.  Of one (sequence, kv head) row j <- row keep[j] with keep ascending,
+// so no source lies before its destination: a CTA takes the rows of one pool in order, a
+// chunk at a time, and stores a chunk once all of it has been loaded; the next chunk's
+// sources lie behind every row stored so far, so its loads need not wait.
+constexpr int kMaxPools = 8;
+struct CompactArgs {
+  unsigned char* pool[kMaxPools];
+  int row_bytes[kMaxPools], unit[kMaxPools];
+  int n_pools;
+  KvAddr addr;
+  const int32_t* keep;
+  int budget;
+  float* weights;  // [B, Hkv, T] or nullptr
+  int T;
+};
+
+constexpr int kCompactThreads = 256, kCompactUnroll = 4;
+
+template <typename U, typename Src, typename Dst>
+__device__ __forceinline__ void compact_rows(int rows, int per, Src src, Dst dst) {
+  const int64_t units = static_cast<int64_t>(rows) * per;
+  for (int64_t base = 0; base < units; base += kCompactThreads * kCompactUnroll) {
+    U v[kCompactUnroll];
+#pragma unroll
+    for (int u = 0; u < kCompactUnroll; ++u) {
+      const int64_t i = base + u * kCompactThreads + threadIdx.x;
+      if (i < units) {
+        const U* p = src(static_cast<int>(i / per), static_cast<int>(i % per));
+        if (p) v[u] = *p;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kCompactUnroll; ++u) {
+      const int64_t i = base + u * kCompactThreads + threadIdx.x;
+      if (i < units) {
+        U* p = dst(static_cast<int>(i / per), static_cast<int>(i % per));
+        if (p) *p = v[u];
+      }
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kCompactThreads) compact_kernel(const CompactArgs a) {
+  const int which = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int64_t bh = static_cast<int64_t>(b) * gridDim.y + h;
+  const int32_t* keep = a.keep + bh * a.budget;
+  // ascending and non-negative, then -1 to the end; anything else leaves the pair untouched
+  int n = 0, bad = 0;
+  for (int j = threadIdx.x; j < a.budget; j += kCompactThreads) {
+    const int k = keep[j], prev = j ? keep[j - 1] : -1;
+    if (k >= 0) {
+      n = j + 1;
+      bad |= k <= prev || (j && prev < 0) || (a.weights && k >= a.T);
+    } else {
+      bad |= k != -1;
+    }
+  }
+  if (__syncthreads_or(bad)) {
+    if (threadIdx.x == 0) spa_raise(SPA_DEVERR_BAD_INDEX);
+    return;
+  }
+  __shared__ int s_n;
+  if (threadIdx.x == 0) s_n = 0;
+  __syncthreads();
+  atomicMax(&s_n, n);
+  __syncthreads();
+  n = s_n;
+  if (which < a.n_pools) {
+    unsigned char* pool = a.pool[which];
+    const int bytes = a.row_bytes[which];
+    const auto at = [&](int t, int off) -> unsigned char* {
+      const int64_t row = a.addr.row(b, h, t);
+      if (row < 0 || row >= a.addr.total_rows) {
+        spa_raise(SPA_DEVERR_BAD_PAGE);
+        return nullptr;
+      }
+      return pool + row * bytes + off;
+    };
+    const auto run = [&](auto unit) {
+      using U = decltype(unit);
+      // a row whose source or destination has no page is left out whole
+      compact_rows<U>(
+          n, bytes / static_cast<int>(sizeof(U)),
+          [&](int j, int u) {
+            return keep[j] == j ? nullptr : reinterpret_cast<const U*>(at(keep[j], u * static_cast<int>(sizeof(U))));
+          },
+          [&](int j, int u) -> U* {
+            if (keep[j] == j || !at(keep[j], 0)) return nullptr;
+            return reinterpret_cast<U*>(at(j, u * static_cast<int>(sizeof(U))));
+          });
+    };
+    switch (a.unit[which]) {
+      case 16: run(uint4{}); break;
+      case 8: run(uint2{}); break;
+      case 4: run(uint32_t{}); break;
+      case 2: run(uint16_t{}); break;
+      default: run(static_cast<unsigned char>(0)); break;
+    }
+  } else if (a.weights) {
+    float* w = a.weights + bh * a.T;
+    compact_rows<float>(
+        n, 1, [&](int j, int) { return static_cast<const float*>(w + keep[j]); }, [&](int j, int) { return w + j; });
+    // the sources behind row n have all been loaded
+    __syncthreads();
+    for (int t = n + threadIdx.x; t < a.T; t += kCompactThreads) w[t] = 0.f;
+  }
+}
+
+}  // namespace spa
+
+extern "C" int spa_select_tokens(const float* weights, int batch, int kv_heads, int tokens, const int32_t* lens,
+                                 int budget, int recent, int32_t* keep, int32_t* kept_lens, spa_stream_t stream) {
+  if (!weights || !lens || !keep || !kept_lens || batch <= 0 || batch > 65535 || kv_heads <= 0 || tokens <= 0 ||
+      budget <= 0 || recent < 0)
+    return SPA_ERR_INVALID;
+  spa::select_tokens_kernel<<<dim3(kv_heads, batch), spa::kSelThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      weights, tokens, lens, budget, recent, keep, kept_lens);
+  SPA_CHECK_CUDA(cudaGetLastError());
+  return SPA_OK;
+}
+
+extern "C" int spa_compact_tokens(const spa_kv_layout* kv, int n_pools, void* const* pools, const int* row_bytes,
+                                  int batch, int kv_heads, const int32_t* keep, int budget, float* weights,
+                                  int weight_tokens, spa_stream_t stream) {
+  if (!kv || !keep || n_pools < 0 || n_pools > spa::kMaxPools || (n_pools > 0 && (!pools || !row_bytes)) ||
+      batch <= 0 || batch > 65535 || kv_heads <= 0 || kv_heads > 65535 || budget <= 0 ||
+      (weights && weight_tokens <= 0) || (n_pools == 0 && !weights))
+    return SPA_ERR_INVALID;
+  if (n_pools > 0 && (kv->page_size <= 0 || kv->total_rows <= 0 || (kv->page_table && kv->table_stride <= 0)))
+    return SPA_ERR_INVALID;
+  spa::CompactArgs a{};
+  for (int i = 0; i < n_pools; ++i) {
+    if (!pools[i] || row_bytes[i] <= 0) return SPA_ERR_INVALID;
+    a.pool[i] = static_cast<unsigned char*>(pools[i]);
+    a.row_bytes[i] = row_bytes[i];
+    const uintptr_t x = reinterpret_cast<uintptr_t>(pools[i]) | static_cast<uintptr_t>(row_bytes[i]);
+    a.unit[i] = x % 16 == 0 ? 16 : x % 8 == 0 ? 8 : x % 4 == 0 ? 4 : x % 2 == 0 ? 2 : 1;
+  }
+  a.n_pools = n_pools;
+  a.addr = make_kv_addr(*kv);
+  a.keep = keep;
+  a.budget = budget;
+  a.weights = weights;
+  a.T = weight_tokens;
+  spa::compact_kernel<<<dim3(n_pools + (weights ? 1 : 0), kv_heads, batch), spa::kCompactThreads, 0,
+                        reinterpret_cast<cudaStream_t>(stream)>>>(a);
+  SPA_CHECK_CUDA(cudaGetLastError());
+  return SPA_OK;
+}

@@ -10,6 +10,9 @@
 #include "session.cuh"
 #include "model.cuh"
 #include "cache.cuh"
+#include "int4.cuh"
+#include "cache_decode.cuh"
+#include "evict.cuh"
 #include "decoder_step.cuh"
 #include "prefill_generic.cuh"
 #include "prefill_sm100.cuh"

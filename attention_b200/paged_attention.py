@@ -22,8 +22,9 @@ import ctypes
 import torch
 
 from . import _lib
-from ._util import (as_int32, as_int64, const_i32, dtype_code, require_contiguous, require_cuda, stream_ptr,
-                    workspace)
+from ._util import (as_int32, as_int64, const_i32, dtype_code, on_device, require_contiguous, require_cuda,
+                    stream_ptr, workspace)
+from .int4 import check_weights
 
 
 def contiguous_layout(keys: torch.Tensor, values: torch.Tensor, page_size: int) -> _lib.KvLayout:
@@ -65,14 +66,34 @@ def _decode(query, kv_layout, kv_heads, context_lens, local_window, selected, to
     return out
 
 
+def _decode_weights(query, layout, kv_heads, lens, tokens, local_window, max_candidates, weights) -> torch.Tensor:
+    batch, q_heads, head_dim = query.shape
+    dev = query.device
+    check_weights(weights, batch, kv_heads, dev)
+    out = torch.empty_like(query)
+    code = dtype_code(query)
+    need = _lib.lib.spa_cache_decode_workspace_size(batch, q_heads, kv_heads, head_dim, max_candidates, tokens, 1, code)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    with on_device(dev):
+        rc = _lib.lib.spa_paged_decode_weights(query.data_ptr(), code, batch, q_heads, kv_heads, head_dim,
+                                               ctypes.byref(layout), lens.data_ptr(), tokens, local_window,
+                                               max_candidates, head_dim ** -0.5, out.data_ptr(), weights.data_ptr(),
+                                               weights.size(2), ws.data_ptr(), need, stream_ptr(dev))
+    _lib.check(rc, "spa_paged_decode_weights")
+    return out
+
+
 def paged_decode_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, *,
                            page_table: torch.Tensor | None = None, context_lens: torch.Tensor | None = None,
-                           local_window: int = 0) -> torch.Tensor:
+                           local_window: int = 0, weights: torch.Tensor | None = None) -> torch.Tensor:
     """Fused attention for q=[B,H,D] over K/V=[B,H,L,D] (reference: triton_paged_attention.py:56).
 
     With ``page_table``, K/V are a page pool ``[num_pages, Hkv, P, D]`` and the
     candidates of sequence b are its first ``context_lens[b]`` tokens (the last
-    ``local_window`` of them when local_window > 0)."""
+    ``local_window`` of them when local_window > 0).
+
+    ``weights`` (fp32 ``[B, Hkv, T]``, in place): each token's probability, summed over its kv
+    head's query heads, is added to it; T covers the contexts (for ``select_tokens``)."""
     if not (query.is_cuda and keys.is_cuda and values.is_cuda):
         raise ValueError("CUDA tensors are required")
     if not (query.is_contiguous() and keys.is_contiguous() and values.is_contiguous()):
@@ -94,6 +115,8 @@ def paged_decode_attention(query: torch.Tensor, keys: torch.Tensor, values: torc
         layout = contiguous_layout(keys, values, length)
         lens = const_i32(query.device, batch, length)
         max_cand = length if local_window <= 0 else min(length, local_window)
+        if weights is not None:
+            return _decode_weights(query, layout, keys.size(1), lens, length, local_window, max_cand, weights)
         return _decode(query, layout, keys.size(1), lens, local_window, None, 0, max_cand, None)
     if context_lens is None:
         raise ValueError("context_lens is required with page_table")
@@ -106,6 +129,9 @@ def paged_decode_attention(query: torch.Tensor, keys: torch.Tensor, values: torc
     max_cand = table.size(1) * keys.size(2)
     if local_window > 0:
         max_cand = min(max_cand, local_window)
+    if weights is not None:
+        return _decode_weights(query, layout, keys.size(1), lens, table.size(1) * keys.size(2), local_window, max_cand,
+                               weights)
     return _decode(query, layout, keys.size(1), lens, local_window, None, 0, max_cand, (table, lens))
 
 

@@ -737,6 +737,85 @@ size_t spa_decoder_step_workspace_size(const spa_decoder_step_params* params);
 int spa_decoder_step(const spa_decoder_step_params* params, spa_stream_t stream);
 
 /*
+ * The 4-bit paged cache.  Addressing is spa_kv_layout's, its "rows" being codes of
+ * head_dim / 2 bytes (k and v point to them); k_scales and v_scales hold 2 * head_dim / 32
+ * fp16 per row.  A row is cut into G = head_dim / 32 groups of 32 values.  For a group with
+ * extremes lo and hi, in fp32 arithmetic: scale = fp16((hi - lo) / 15), zero = fp16(lo), both
+ * clamped to +-65504; n = clamp(rint((x - zero) / scale), 0, 15), 0 where scale is 0; it
+ * stands for scale * n + zero.  A group that holds a NaN or an infinity reads back as NaN.
+ *   codes  [pages, Hkv, P, D / 2]  value d = 32 j + 4 g + i is nibble i (low bits first) of
+ *                                  the row's little-endian 16-bit word g * G + j
+ *   scales [pages, Hkv, P, 2, G]   the row's scales, then its zeros
+ * head_dim is a multiple of 32 up to 256; the four arrays are 16-byte aligned.
+ *
+ * spa_int4_append writes tokens positions[b] + t, t < (new_lens ? new_lens[b] : tokens), from
+ * k_new / v_new, whose element (b, h, t, d) lies at b * stride_b + h * stride_h +
+ * t * stride_t + d.  A sequence's negative tokens are skipped; a token without a page is
+ * skipped and raises device error bit 2.
+ * spa_int4_read writes the same tokens' values to k_out / v_out [B, Hkv, tokens, D]: zeros
+ * past lens[b] and where spa_int4_append would have skipped the token.
+ * No reference counterpart (the reference keeps K/V in the model's dtype).
+ */
+int spa_int4_append(const spa_kv_layout* kv, void* k_scales, void* v_scales, int dtype, int batch, int kv_heads,
+                    int head_dim, int tokens, const void* k_new, const void* v_new, int64_t stride_b,
+                    int64_t stride_h, int64_t stride_t, const int32_t* positions, const int32_t* new_lens,
+                    spa_stream_t stream);
+int spa_int4_read(const spa_kv_layout* kv, const void* k_scales, const void* v_scales, int dtype, int batch,
+                  int kv_heads, int head_dim, int tokens, const int32_t* positions, const int32_t* lens, void* k_out,
+                  void* v_out, spa_stream_t stream);
+
+/*
+ * Decode attention over the 4-bit cache: the candidates and rules of spa_paged_decode
+ * (dense, local window, or local window and selected pages), for queries and outputs of
+ * `dtype`.  max_tokens is what a sequence can hold (table_stride * page_size, or its
+ * contiguous length); a longer context raises device error bit 2 and is cut.
+ *
+ * weights (NULL, or fp32 [batch, kv_heads, weight_tokens]; not with `selected`): every
+ * candidate token's softmax probability, summed over the query heads of its kv head, is
+ * added to it.  Candidates at or past weight_tokens are not, and raise bit 4.  The sum has
+ * one fixed order.
+ *
+ * spa_paged_decode_weights: spa_paged_decode's dense and local-window forms of a plain
+ * cache with that accumulation.
+ *
+ * Workspace: spa_cache_decode_workspace_size bytes, 16-byte aligned, with any contents; its
+ * kv_dtype is the plain cache's, or -1 for the 4-bit cache.  Calls that may overlap need
+ * workspaces of their own.  At most 256 query heads per kv head.
+ */
+size_t spa_cache_decode_workspace_size(int batch, int q_heads, int kv_heads, int head_dim, int max_candidates,
+                                       int max_tokens, int weights, int kv_dtype);
+int spa_int4_decode(const void* q, int dtype, int batch, int q_heads, int kv_heads, int head_dim,
+                    const spa_kv_layout* kv, const void* k_scales, const void* v_scales, const int32_t* context_lens,
+                    int max_tokens, int local_window, const int64_t* selected, int top_m, int max_candidates,
+                    double scale, void* out, float* weights, int weight_tokens, void* workspace,
+                    size_t workspace_bytes, spa_stream_t stream);
+int spa_paged_decode_weights(const void* q, int dtype, int batch, int q_heads, int kv_heads, int head_dim,
+                             const spa_kv_layout* kv, const int32_t* context_lens, int max_tokens, int local_window,
+                             int max_candidates, double scale, void* out, float* weights, int weight_tokens,
+                             void* workspace, size_t workspace_bytes, spa_stream_t stream);
+
+/*
+ * Eviction.  spa_select_tokens: which tokens of each (sequence, kv head) stay, from weights
+ * [batch, kv_heads, tokens].  With L = min(lens[b], tokens): all of them while L <= budget;
+ * else the last min(recent, budget) and, of the others, those of the largest weight, ties to
+ * the lower token (a NaN is below every number).  keep [batch, kv_heads, budget] holds them in
+ * ascending order, then -1; kept_lens[b] = min(L, budget).
+ *
+ * spa_compact_tokens: moves row keep[j] to token j, j = 0, 1, ..., in place, in each of the
+ * n_pools (up to 8) pools; row_bytes[i] is the size of a row of pools[i], addressed by kv's
+ * geometry (its k and v are not used).  weights, when given, move along and are zero behind
+ * the kept tokens.  Rows of the pools behind the kept tokens stay as they were.  keep must be
+ * ascending and then -1, with no token twice; a (sequence, kv head) whose list is not is left
+ * as it was and raises device error bit 4.  A row without a page is left out (bit 2).
+ * No two sequences may share a page that either of them moves rows in.
+ */
+int spa_select_tokens(const float* weights, int batch, int kv_heads, int tokens, const int32_t* lens, int budget,
+                      int recent, int32_t* keep, int32_t* kept_lens, spa_stream_t stream);
+int spa_compact_tokens(const spa_kv_layout* kv, int n_pools, void* const* pools, const int* row_bytes, int batch,
+                       int kv_heads, const int32_t* keep, int budget, float* weights, int weight_tokens,
+                       spa_stream_t stream);
+
+/*
  * Diagnostic for the failure path: one kernel waits on an mbarrier that nothing
  * completes, with the library's bounded wait limited to `cycles` (1 .. 4e9 clock
  * cycles).  The wait gives up, the kernel returns, and spa_device_error then reports
