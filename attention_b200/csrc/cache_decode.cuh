@@ -11,98 +11,10 @@
 // final log-sum-exp; the finish kernel turns them into probabilities and adds them up.
 #pragma once
 
-#include "decode.cuh"
-#include "int4.cuh"
+#include "cache_args.cuh"
+#include "int4_mma.cuh"
 
 namespace spa {
-
-struct CacheDecodeArgs {
-  const void* q;
-  void* out;
-  int dtype;  // of q and out
-  int B, Hq, Hkv, group, D;
-  const void* k;
-  const void* v;
-  const __half* k_scales;
-  const __half* v_scales;
-  KvAddr addr;
-  const int32_t* ctx_lens;
-  int cap;  // tokens a sequence can hold
-  int local_window;
-  const int64_t* selected;
-  int top_m;
-  int heads, chunks;  // query heads a CTA serves, CTAs per kv head
-  int nsplit;
-  float scale_log2;
-  float* part_o;    // [B*Hq, nsplit, D]
-  float* part_lse;  // [B*Hq, nsplit]
-  float* scores;    // [B, Hkv, cap, group] or nullptr
-  float* weights;   // [B, Hkv, T] or nullptr
-  int T;
-};
-
-__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
-  return dtype == SPA_F32   ? static_cast<const float*>(p)[i]
-         : dtype == SPA_F16 ? __half2float(static_cast<const __half*>(p)[i])
-                            : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
-__device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float x) {
-  if (dtype == SPA_F32)
-    static_cast<float*>(p)[i] = x;
-  else if (dtype == SPA_F16)
-    static_cast<__half*>(p)[i] = __float2half_rn(x);
-  else
-    static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
-}
-
-// Tiles of TILE tokens: the window (or the whole context), then each selected page.
-struct TilePlan {
-  int ctx, lo, seg, n_seg, cpp, n;
-};
-template <int TILE>
-__device__ __forceinline__ TilePlan tile_plan(const CacheDecodeArgs& a, int b) {
-  TilePlan p;
-  const int ctx = a.ctx_lens[b];
-  if (ctx > a.cap) spa_raise(SPA_DEVERR_BAD_PAGE);  // tokens no page of the table row can hold
-  p.ctx = min(max(ctx, 0), a.cap);
-  p.lo = a.selected || a.local_window > 0 ? max(0, p.ctx - a.local_window) : 0;
-  p.seg = p.lo / TILE * TILE;
-  p.n_seg = p.ctx > p.lo ? (p.ctx - p.seg + TILE - 1) / TILE : 0;
-  p.cpp = (a.addr.page_size + TILE - 1) / TILE;
-  p.n = p.n_seg + (a.selected ? a.top_m * p.cpp : 0);
-  return p;
-}
-// Token of slot `i` of tile `tile`, or -1 (not a candidate).
-template <int TILE>
-__device__ __forceinline__ int tile_token(const CacheDecodeArgs& a, const TilePlan& p, int b, int tile, int i) {
-  if (tile < p.n_seg) {
-    const int t = p.seg + tile * TILE + i;
-    return t >= p.lo && t < p.ctx ? t : -1;
-  }
-  const int kk = tile - p.n_seg, j = kk / p.cpp, o = (kk - j * p.cpp) * TILE + i;
-  const int64_t lp = a.selected[static_cast<int64_t>(b) * a.top_m + j];
-  if (lp < 0) return -1;  // an empty slot
-  if (lp >= p.ctx || lp * a.addr.page_size >= p.ctx) {
-    if (i == 0) spa_raise(SPA_DEVERR_BAD_PAGE);
-    return -1;
-  }
-  const int64_t t = lp * a.addr.page_size + o;
-  return o < a.addr.page_size && t < p.ctx ? static_cast<int>(t) : -1;
-}
-// Row of a token, or -1.
-__device__ __forceinline__ int64_t token_row(const CacheDecodeArgs& a, int b, int h, int t) {
-  if (t < 0) return -1;
-  const int64_t row = a.addr.row(b, h, t);
-  if (row < 0 || row >= a.addr.total_rows) {
-    spa_raise(SPA_DEVERR_BAD_PAGE);
-    return -1;
-  }
-  return row;
-}
-__device__ __forceinline__ void split_range(int n, int split, int nsplit, int& t0, int& t1) {
-  t0 = static_cast<int>(static_cast<int64_t>(n) * split / nsplit);
-  t1 = static_cast<int>(static_cast<int64_t>(n) * (split + 1) / nsplit);
-}
 
 // ---------------------------------------------------------------------------
 // CUDA-core kernel: any head_dim up to 256, any cache type.  Lane l holds the values
@@ -144,7 +56,8 @@ __global__ void __launch_bounds__(kPlainWarps * 32) cache_decode_plain_kernel(co
   };
   for (int tile = t0 + warp; tile < t1; tile += kPlainWarps) {
     const int tok = tile_token<32>(a, p, b, tile, lane);
-    const int64_t my_row = token_row(a, b, h, tok);
+    int ahead;
+    const int64_t my_row = token_row(a, b, h, tok, p.ctx, ahead);
     unsigned live = __ballot_sync(0xffffffffu, my_row >= 0);
     if (a.scores && tok >= 0 && my_row < 0)
       for (int n = 0; n < heads; ++n)
@@ -270,27 +183,33 @@ __global__ void __launch_bounds__(kFinishThreads) cache_decode_finish_kernel(con
 
 // ---------------------------------------------------------------------------
 // host planning
+constexpr int kCacheCtasPerSm = 4;
 struct CachePlan {
-  bool fast;
+  bool mma;
   int heads, chunks, nsplit;
 };
-inline CachePlan cache_plan(int batch, int q_heads, int kv_heads, int head_dim, int max_candidates, bool int4,
-                            int cache_dtype) {
+inline CachePlan cache_plan(int batch, int q_heads, int kv_heads, int head_dim, int max_candidates, int kv_dtype,
+                            bool mma) {
   CachePlan p;
-  (void)head_dim;
-  (void)int4;
-  (void)cache_dtype;
   const int group = q_heads / kv_heads;
-  p.fast = false;
-  p.heads = kPlainHeads;
+  p.mma = mma;
+  const int warps = mma ? kI4Warps : kPlainWarps;
+  p.heads = mma ? int4_mma_heads(head_dim, group) : kPlainHeads;
   p.chunks = (group + p.heads - 1) / p.heads;
+  (void)kv_dtype;
+  // the split count that ends first: waves of CTAs times a CTA's tiles (32 tokens a warp) and
+  // what a CTA costs besides them, about kCtaTiles tiles
+  constexpr int64_t kCtaTiles = 4;
   const int64_t ctas = static_cast<int64_t>(batch) * kv_heads * p.chunks;
-  const int64_t slots = device_sm_count() * 4;
-  const int64_t most = max_candidates / 32 / kPlainWarps + 1;
-  int64_t ns = slots / ctas;
-  if (ns > most) ns = most;
-  if (ns > 64) ns = 64;
-  p.nsplit = ns < 1 ? 1 : static_cast<int>(ns);
+  const int64_t slots = static_cast<int64_t>(device_sm_count()) * kCacheCtasPerSm;
+  const int64_t tiles = (max_candidates + 31) / 32 + 1;
+  int64_t best = 0;
+  p.nsplit = 1;
+  for (int64_t ns = 1; ns <= 64 && (ns == 1 || ns * warps < tiles + warps); ++ns) {
+    const int64_t each = (tiles + ns * warps - 1) / (ns * warps);
+    const int64_t cost = (ctas * ns + slots - 1) / slots * (each + kCtaTiles);
+    if (ns == 1 || cost < best) best = cost, p.nsplit = static_cast<int>(ns);
+  }
   return p;
 }
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -332,10 +251,12 @@ int cache_decode_impl(CacheDecodeArgs a, int kv_dtype, const spa_kv_layout* kv, 
       max_candidates < 0 || a.cap <= 0 || a.local_window < 0)
     return SPA_ERR_INVALID;
   if (kv->page_size <= 0 || kv->total_rows <= 0 || (kv->page_table && kv->table_stride <= 0)) return SPA_ERR_INVALID;
+  if (!(scale > 0.0) || scale > 1e30) return SPA_ERR_INVALID;
   if ((a.selected && a.top_m <= 0) || (a.weights && (a.T <= 0 || a.selected))) return SPA_ERR_INVALID;
   a.group = a.Hq / a.Hkv;
   if (a.group > 256) return SPA_ERR_UNSUPPORTED;
-  const CachePlan p = cache_plan(a.B, a.Hq, a.Hkv, a.D, max_candidates, kv_dtype < 0, kv_dtype);
+  const CachePlan p = cache_plan(a.B, a.Hq, a.Hkv, a.D, max_candidates, kv_dtype,
+                                 kv_dtype < 0 && int4_mma_serves(a.D, kv->total_rows));
   if (static_cast<int64_t>(a.Hkv) * p.chunks > 65535) return SPA_ERR_UNSUPPORTED;
   const CacheScratch s = cache_scratch(p, a.B, a.Hq, a.D, a.cap, a.weights != nullptr);
   if (s.total && (!workspace || workspace_bytes < s.total || reinterpret_cast<uintptr_t>(workspace) % 16))
@@ -343,6 +264,8 @@ int cache_decode_impl(CacheDecodeArgs a, int kv_dtype, const spa_kv_layout* kv, 
   a.k = kv->k;
   a.v = kv->v;
   a.addr = make_kv_addr(*kv);
+  a.page_inv = 0xffffffffu / static_cast<uint32_t>(kv->page_size);
+  a.q_vec = reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
   a.heads = p.heads;
   a.chunks = p.chunks;
   a.nsplit = p.nsplit;
@@ -354,7 +277,9 @@ int cache_decode_impl(CacheDecodeArgs a, int kv_dtype, const spa_kv_layout* kv, 
   a.scores = a.weights ? reinterpret_cast<float*>(ws + s.scores) : nullptr;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   int rc;
-  if (kv_dtype < 0)
+  if (p.mma)
+    rc = launch_int4_decode(a, st);
+  else if (kv_dtype < 0)
     rc = launch_cache_plain<uint8_t>(a, st);
   else if (kv_dtype == SPA_F32)
     rc = launch_cache_plain<float>(a, st);
@@ -376,8 +301,14 @@ extern "C" size_t spa_cache_decode_workspace_size(int batch, int q_heads, int kv
   if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0 || max_candidates < 0 ||
       max_tokens <= 0)
     return 0;
-  const spa::CachePlan p = spa::cache_plan(batch, q_heads, kv_heads, head_dim, max_candidates, kv_dtype < 0, kv_dtype);
-  return spa::cache_scratch(p, batch, q_heads, head_dim, max_tokens, weights != 0).total;
+  // the number of rows decides between the kernels, and it is not known here: the larger need
+  size_t most = 0;
+  for (int mma = 0; mma < 2; ++mma) {
+    const spa::CachePlan p = spa::cache_plan(batch, q_heads, kv_heads, head_dim, max_candidates, kv_dtype, mma != 0);
+    const size_t need = spa::cache_scratch(p, batch, q_heads, head_dim, max_tokens, weights != 0).total;
+    most = need > most ? need : most;
+  }
+  return most;
 }
 
 extern "C" int spa_int4_decode(const void* q, int dtype, int batch, int q_heads, int kv_heads, int head_dim,
