@@ -24,11 +24,11 @@ struct CacheDecodeArgs {
   int local_window;
   const int64_t* selected;
   int top_m;
-  int heads, chunks;  // query heads a CTA serves, CTAs per kv head
-  int nsplit;
+  int heads, chunks;  // query heads a CTA serves, such chunks per kv head
+  int ctas;           // CTAs that share all tiles out evenly; 0: one CTA per pair
   float scale_log2;
-  float* part_o;    // [B*Hq, nsplit, D]
-  float* part_lse;  // [B*Hq, nsplit]
+  float* part_o;    // [slots, heads, D]
+  float* part_lse;  // [slots, heads]
   float* scores;    // [B, Hkv, cap, group] or nullptr
   float* weights;   // [B, Hkv, T] or nullptr
   int T;
@@ -66,6 +66,22 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float x
   else
     static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
 }
+__device__ __forceinline__ void store4_any(void* p, int dtype, int64_t i, float4 x) {  // rows of 16 bytes' multiples
+  if (dtype == SPA_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = x;
+  } else if (dtype == SPA_F16) {
+    const __half2 v[2] = {__floats2half2_rn(x.x, x.y), __floats2half2_rn(x.z, x.w)};
+    *reinterpret_cast<uint2*>(static_cast<__half*>(p) + i) = *reinterpret_cast<const uint2*>(v);
+  } else {
+    const __nv_bfloat162 v[2] = {__floats2bfloat162_rn(x.x, x.y), __floats2bfloat162_rn(x.z, x.w)};
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p) + i) = *reinterpret_cast<const uint2*>(v);
+  }
+}
+// a * b / c, in 32 bits where the product fits
+__device__ __forceinline__ int64_t mul_div(int64_t a, int b, int64_t c) {
+  const int64_t p = a * b;
+  return (p | c) >> 32 ? p / c : static_cast<int64_t>(static_cast<uint32_t>(p) / static_cast<uint32_t>(c));
+}
 
 // Tiles of TILE tokens: the window (or the whole context), then each selected page.
 struct TilePlan {
@@ -101,26 +117,132 @@ __device__ __forceinline__ int tile_token(const CacheDecodeArgs& a, const TilePl
   const int64_t t = lp * a.addr.page_size + o;
   return o < a.addr.page_size && t < p.ctx ? static_cast<int>(t) : -1;
 }
-// Row of a token, or -1; `ahead`: the tokens from it on that share its page and are in the context.
-__device__ __forceinline__ int64_t token_row(const CacheDecodeArgs& a, int b, int h, int t, int ctx, int& ahead) {
-  ahead = 0;
-  if (t < 0) return -1;
+// Physical page of a token (t >= 0) or -1, and the token's place in it.
+__device__ __forceinline__ int token_page(const CacheDecodeArgs& a, int b, int t, int& off) {
   // the multiply falls short by at most one
-  int lp = static_cast<int>(__umulhi(static_cast<uint32_t>(t), a.page_inv)), off = t - lp * a.addr.page_size;
+  int lp = static_cast<int>(__umulhi(static_cast<uint32_t>(t), a.page_inv));
+  off = t - lp * a.addr.page_size;
   if (off >= a.addr.page_size) ++lp, off -= a.addr.page_size;
-  const int64_t pg = a.addr.page_of(b, lp);
-  const int64_t row =
-      pg < 0 ? -1 : b * a.addr.batch_stride_rows + pg * a.addr.page_stride_rows + h * a.addr.head_stride_rows + off;
-  if (row < 0 || row >= a.addr.total_rows) {
+  if (!a.addr.page_table) return lp;
+  return lp < a.addr.table_stride ? a.addr.page_table[static_cast<int64_t>(b) * a.addr.table_stride + lp] : -1;
+}
+// Row of a token in its page, or -1.
+__device__ __forceinline__ int64_t page_row(const CacheDecodeArgs& a, int b, int h, int t, int page, int off) {
+  if (t < 0) return -1;
+  const int64_t row = b * a.addr.batch_stride_rows + page * a.addr.page_stride_rows + h * a.addr.head_stride_rows + off;
+  if (page < 0 || row < 0 || row >= a.addr.total_rows) {
     spa_raise(SPA_DEVERR_BAD_PAGE);
     return -1;
   }
-  ahead = min(a.addr.page_size - off, ctx - t);
   return row;
 }
 __device__ __forceinline__ void split_range(int n, int split, int nsplit, int& t0, int& t1) {
   t0 = static_cast<int>(static_cast<int64_t>(n) * split / nsplit);
   t1 = static_cast<int>(static_cast<int64_t>(n) * (split + 1) / nsplit);
+}
+
+// ---- Sharing out the work.  A pair is a (sequence, kv head, chunk of its query heads); all of a
+// sequence's pairs have its number of tiles.  The pairs' tiles, end to end, are cut into `ctas`
+// equal ranges, one a CTA, however the lengths are spread; a range may end inside a pair, so a
+// pair's results are partials of consecutive CTAs, in slot CTA + pair (both only ever grow along
+// the ranges, so no two share a slot).  A pair that one CTA covers whole needs no partial.
+constexpr int kFlatBatch = 1024;  // longest batch whose prefix sums a CTA makes for itself
+
+// pre[b] = tiles of one pair of each sequence before b, pre[B] the total; every thread calls it.
+template <int TILE>
+__device__ __forceinline__ void tiles_before(const CacheDecodeArgs& a, int* pre) {
+  const int lane = threadIdx.x & 31;
+  if (a.B <= 32) {
+    if (threadIdx.x < 32) {
+      int x = lane < a.B ? tile_plan<TILE>(a, lane).n : 0;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, off);
+        if (lane >= off) x += y;
+      }
+      pre[lane + 1] = x;
+      if (lane == 0) pre[0] = 0;
+    }
+    __syncthreads();
+    return;
+  }
+  for (int b = threadIdx.x; b < a.B; b += blockDim.x) pre[b + 1] = tile_plan<TILE>(a, b).n;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    int sum = 0;
+    for (int base = 0; base < a.B; base += 32) {
+      int x = base + lane < a.B ? pre[base + lane + 1] : 0;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, off);
+        if (lane >= off) x += y;
+      }
+      if (base + lane < a.B) pre[base + lane + 1] = sum + x;
+      sum += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) pre[0] = 0;
+  }
+  __syncthreads();
+}
+struct Segment {
+  int b, h, chunk, u0, u1;  // tiles [u0, u1) of a pair
+  int slot;
+  bool whole;  // all of the pair's tiles
+};
+// The range [x, x1) of this CTA, cut at the pairs' ends: one segment a call.
+struct Work {
+  int64_t x, x1;
+  __device__ __forceinline__ Work(const CacheDecodeArgs& a, const int* pre) {
+    const int64_t total = static_cast<int64_t>(a.ctas ? pre[a.B] : 0) * a.Hkv * a.chunks;
+    x = a.ctas ? mul_div(total, blockIdx.x, a.ctas) : 0;
+    x1 = a.ctas ? mul_div(total, blockIdx.x + 1, a.ctas) : 1;
+  }
+  template <int TILE>
+  __device__ __forceinline__ bool next(const CacheDecodeArgs& a, const int* pre, Segment& s) {
+    if (x >= x1) return false;
+    const int pairs = a.Hkv * a.chunks;
+    int pair = blockIdx.x;
+    if (a.ctas) {
+      int lo = 0, hi = a.B;  // the last sequence that starts at or before x and is not empty
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (static_cast<int64_t>(pre[mid]) * pairs <= x)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      const int n = pre[lo + 1] - pre[lo];
+      const int64_t y = x - static_cast<int64_t>(pre[lo]) * pairs;
+      const int hc = static_cast<int>(mul_div(y, 1, n));
+      s.u0 = static_cast<int>(y - static_cast<int64_t>(hc) * n);
+      s.u1 = static_cast<int>(min(static_cast<int64_t>(n), s.u0 + (x1 - x)));
+      s.whole = s.u1 - s.u0 == n;
+      x += s.u1 - s.u0;
+      pair = lo * pairs + hc;
+    } else {
+      s.u0 = 0;
+      s.u1 = tile_plan<TILE>(a, pair / pairs).n;
+      s.whole = true;
+      x = x1;
+    }
+    s.slot = blockIdx.x + pair;
+    s.b = pair / pairs;
+    pair -= s.b * pairs;
+    s.h = pair / a.chunks;
+    s.chunk = pair - s.h * a.chunks;
+    return true;
+  }
+};
+// CTAs [first, last] that hold tiles [at, at + n) of all `total`, n > 0
+__device__ __forceinline__ void ctas_of(int64_t at, int n, int64_t total, int ctas, int& first, int& last) {
+  // the last CTA whose range starts at or before tile x: the largest i with total i / ctas <= x
+  const auto cta = [&](int64_t x) {
+    const int64_t p = (x + 1) * ctas - 1;
+    return static_cast<int>((p | total) >> 32 ? p / total
+                                              : static_cast<int64_t>(static_cast<uint32_t>(p) / static_cast<uint32_t>(total)));
+  };
+  first = cta(at);
+  last = cta(at + n - 1);
 }
 
 }  // namespace spa

@@ -3,9 +3,9 @@
 //
 // The candidates of a sequence (its context, its local window, or window and selected pages)
 // are cut into tiles that never straddle a selected page; the tiles of one (sequence, kv
-// head) are shared out over `nsplit` CTAs and, inside a CTA, over its warps, each of which
-// keeps its own running maximum and sum.  A CTA merges its warps in shared memory; splits
-// leave (output, log2-sum-exp) partials that cache_decode_finish_kernel joins.  With weights
+// head) are shared out over CTAs (cache_args.cuh) and, inside a CTA, over its warps, each of
+// which keeps its own running maximum and sum.  A CTA merges its warps in shared memory; CTAs
+// that share a pair leave (output, log2-sum-exp) partials that cache_decode_finish_kernel joins.  With weights
 // the scores are kept as well (fp32, one per query head and token: 16 bytes a token at four
 // heads per kv head, against 160 or 512 of K and V), because a token's weight needs the
 // final log-sum-exp; the finish kernel turns them into probabilities and adds them up.
@@ -23,9 +23,14 @@ constexpr int kPlainHeads = 4, kPlainWarps = 4;
 
 template <typename T, int E>  // T = uint8_t: the 4-bit cache
 __global__ void __launch_bounds__(kPlainWarps * 32) cache_decode_plain_kernel(const CacheDecodeArgs a) {
-  const int split = blockIdx.x, h = blockIdx.y / a.chunks, chunk = blockIdx.y % a.chunks, b = blockIdx.z;
+  __shared__ float sm[kPlainWarps][kPlainHeads], sl[kPlainWarps][kPlainHeads], so[kPlainWarps][kPlainHeads][E * 32];
+  __shared__ int pre[kFlatBatch + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = a.D;
-  const int head0 = chunk * kPlainHeads, heads = min(kPlainHeads, a.group - head0);
+  if (a.ctas) tiles_before<32>(a, pre);
+  Work work(a, pre);
+  Segment seg;
+  while (work.next<32>(a, pre, seg)) {
+  const int b = seg.b, h = seg.h, head0 = seg.chunk * kPlainHeads, heads = min(kPlainHeads, a.group - head0);
   const int64_t q0 = static_cast<int64_t>(b) * a.Hq + h * a.group + head0;
   float q[kPlainHeads][E], acc[kPlainHeads][E], m[kPlainHeads], l[kPlainHeads];
 #pragma unroll
@@ -40,8 +45,6 @@ __global__ void __launch_bounds__(kPlainWarps * 32) cache_decode_plain_kernel(co
     }
   }
   const TilePlan p = tile_plan<32>(a, b);
-  int t0, t1;
-  split_range(p.n, split, a.nsplit, t0, t1);
   const auto value = [&](const void* base, const __half* scales, int64_t row, int e) -> float {
     const int d = lane + 32 * e;
     if constexpr (sizeof(T) == 1) {
@@ -54,10 +57,11 @@ __global__ void __launch_bounds__(kPlainWarps * 32) cache_decode_plain_kernel(co
       return d < D ? to_f32<T>(static_cast<const T*>(base)[row * D + d]) : 0.f;
     }
   };
-  for (int tile = t0 + warp; tile < t1; tile += kPlainWarps) {
+  for (int tile = seg.u0 + warp; tile < seg.u1; tile += kPlainWarps) {
     const int tok = tile_token<32>(a, p, b, tile, lane);
-    int ahead;
-    const int64_t my_row = token_row(a, b, h, tok, p.ctx, ahead);
+    int off = 0;
+    const int page = tok < 0 ? -1 : token_page(a, b, tok, off);
+    const int64_t my_row = page_row(a, b, h, tok, page, off);
     unsigned live = __ballot_sync(0xffffffffu, my_row >= 0);
     if (a.scores && tok >= 0 && my_row < 0)
       for (int n = 0; n < heads; ++n)
@@ -99,7 +103,6 @@ __global__ void __launch_bounds__(kPlainWarps * 32) cache_decode_plain_kernel(co
     }
   }
   // merge the warps
-  __shared__ float sm[kPlainWarps][kPlainHeads], sl[kPlainWarps][kPlainHeads], so[kPlainWarps][kPlainHeads][E * 32];
 #pragma unroll
   for (int n = 0; n < kPlainHeads; ++n) {
     if (lane == 0) sm[warp][n] = m[n], sl[warp][n] = l[n];
@@ -117,59 +120,123 @@ __global__ void __launch_bounds__(kPlainWarps * 32) cache_decode_plain_kernel(co
       O = fmaf(so[w][n][d], f, O);
     }
     const float o = W == 0.f ? 0.f : O / W;
-    if (a.part_o) {
-      a.part_o[((q0 + n) * a.nsplit + split) * D + d] = o;
-      if (d == 0) a.part_lse[(q0 + n) * a.nsplit + split] = W == 0.f ? -INFINITY : M + log2f(W);
+    if (a.weights || !seg.whole) {
+      a.part_o[(static_cast<int64_t>(seg.slot) * kPlainHeads + n) * D + d] = o;
+      if (d == 0) a.part_lse[static_cast<int64_t>(seg.slot) * kPlainHeads + n] = W == 0.f ? -INFINITY : M + log2f(W);
     } else {
       store_any(a.out, a.dtype, (q0 + n) * D + d, o);
     }
   }
+  __syncthreads();  // the next segment reuses the buffers
+  }
 }
 
 // ---------------------------------------------------------------------------
-// Joins the splits and, with weights, adds every token's probabilities to its weight.
-// Grid (group + token blocks, Hkv, B): block x < group merges one head's output.
-constexpr int kFinishThreads = 256, kFinishTokens = 1024;
+// Joins the partials and, with weights, adds every token's probabilities to its weight.
+// Grid (head blocks + token blocks, Hkv, B): a warp of the first blocks merges one head's output.
+constexpr int kFinishThreads = 256, kFinishTokens = 1024, kFinishHeads = kFinishThreads / 32;
 
+template <int TILE>
 __global__ void __launch_bounds__(kFinishThreads) cache_decode_finish_kernel(const CacheDecodeArgs a) {
-  pdl_block();
-  const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, ns = a.nsplit;
-  const int64_t q0 = static_cast<int64_t>(b) * a.Hq + h * a.group;
+  const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int pairs = a.Hkv * a.chunks, head_blocks = (a.group + kFinishHeads - 1) / kFinishHeads;
   __shared__ float s_lse[256];
-  if (blockIdx.x < a.group) {
-    const int64_t bh = q0 + blockIdx.x;
-    float M = -INFINITY, W = 0.f;
-    for (int s = 0; s < ns; ++s) M = fmaxf(M, a.part_lse[bh * ns + s]);
-    for (int s = 0; s < ns; ++s) {
-      const float x = a.part_lse[bh * ns + s];
-      W += x == -INFINITY ? 0.f : exp2f(x - M);
+  __shared__ int s_sum[kFinishThreads / 32][2];
+  // this sequence's tiles, those before it, and all
+  const TilePlan plan = tile_plan<TILE>(a, b);
+  int64_t before = 0, total = 0;
+  if (a.ctas) {
+    int x = 0, y = 0;
+    for (int i = tid; i < a.B; i += kFinishThreads) {
+      const int n = tile_plan<TILE>(a, i).n;
+      y += n;
+      if (i < b) x += n;
     }
-    for (int d = tid; d < a.D; d += kFinishThreads) {
-      float O = 0.f;
-      for (int s = 0; s < ns; ++s) {
-        const float x = a.part_lse[bh * ns + s];
-        if (x != -INFINITY) O = fmaf(a.part_o[(bh * ns + s) * a.D + d], exp2f(x - M), O);
+    x = __reduce_add_sync(0xffffffffu, x);
+    y = __reduce_add_sync(0xffffffffu, y);
+    if (lane == 0) s_sum[warp][0] = x, s_sum[warp][1] = y;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kFinishThreads / 32; ++w) before += s_sum[w][0], total += s_sum[w][1];
+  }
+  // log2-sum-exp of head n of the group over its partials first .. last (rows `row` of their
+  // slots); `mine` is this lane's partial of each 32
+  int first = 0, last = -1, row = 0;
+  const auto lse_of = [&](int n) -> float {
+    const int hc = h * a.chunks + n / a.heads, pair = b * pairs + hc;
+    row = n % a.heads;
+    first = last = pair;
+    if (a.ctas)
+      ctas_of(before * pairs + static_cast<int64_t>(hc) * plan.n, plan.n, total * pairs, a.ctas, first, last);
+    first += pair, last += pair;
+    if (first == last && !a.weights) return 0.f;  // its CTA has written the output
+    float M = -INFINITY;
+    for (int s = first + lane; s <= last; s += 32) M = fmaxf(M, a.part_lse[static_cast<int64_t>(s) * a.heads + row]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    float sum = 0.f;
+    for (int s = first + lane; s <= last; s += 32) {
+      const float x = a.part_lse[static_cast<int64_t>(s) * a.heads + row];
+      sum += x == -INFINITY ? 0.f : exp2f(x - M);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    return sum == 0.f ? INFINITY : M + log2f(sum);
+  };
+  pdl_block();
+  if (blockIdx.x < head_blocks) {
+    const int n = blockIdx.x * kFinishHeads + warp;
+    if (n >= a.group) return;
+    const int64_t out = (static_cast<int64_t>(b) * a.Hq + h * a.group + n) * a.D;
+    if (plan.n == 0) {
+      for (int d = lane; d < a.D; d += 32) store_any(a.out, a.dtype, out + d, 0.f);
+      return;
+    }
+    const float lse = lse_of(n);
+    if (first == last && !a.weights) return;
+    // eight partials' loads in flight; four columns a lane where rows allow
+    const auto columns = [&](auto vec) {
+      constexpr int V = decltype(vec)::value;
+      for (int d = lane * V; d < a.D; d += 32 * V) {
+        float o[V] = {};
+        for (int s0 = first; s0 <= last; s0 += 8) {
+          float v[8][V], x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int64_t at = static_cast<int64_t>(min(s0 + i, last)) * a.heads + row;
+            x[i] = s0 + i <= last ? a.part_lse[at] : -INFINITY;
+            if constexpr (V == 4)
+              *reinterpret_cast<float4*>(v[i]) = *reinterpret_cast<const float4*>(a.part_o + at * a.D + d);
+            else
+              v[i][0] = a.part_o[at * a.D + d];
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (x[i] != -INFINITY) {
+              const float f = exp2f(x[i] - lse);
+#pragma unroll
+              for (int e = 0; e < V; ++e) o[e] = fmaf(v[i][e], f, o[e]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) store_any(a.out, a.dtype, out + d + e, o[e]);
       }
-      store_any(a.out, a.dtype, bh * a.D + d, W == 0.f ? 0.f : O / W);
-    }
+    };
+    if (a.D % 4 == 0)
+      columns(std::integral_constant<int, 4>{});
+    else
+      columns(std::integral_constant<int, 1>{});
     return;
   }
-  const int ctx = min(max(a.ctx_lens[b], 0), a.cap);
-  const int lo = a.local_window > 0 ? max(0, ctx - a.local_window) : 0;
-  const int t0 = lo + (blockIdx.x - a.group) * kFinishTokens;
-  if (t0 >= ctx) return;
-  for (int n = tid; n < a.group; n += kFinishThreads) {
-    float M = -INFINITY, W = 0.f;
-    for (int s = 0; s < ns; ++s) M = fmaxf(M, a.part_lse[(q0 + n) * ns + s]);
-    for (int s = 0; s < ns; ++s) {
-      const float x = a.part_lse[(q0 + n) * ns + s];
-      W += x == -INFINITY ? 0.f : exp2f(x - M);
-    }
-    s_lse[n] = W == 0.f ? INFINITY : M + log2f(W);
+  const int t0 = plan.lo + (blockIdx.x - head_blocks) * kFinishTokens;
+  if (t0 >= plan.ctx) return;
+  for (int n = warp; n < a.group; n += kFinishThreads / 32) {
+    const float lse = lse_of(n);
+    if (lane == 0) s_lse[n] = lse;
   }
   __syncthreads();
   const int64_t bh = static_cast<int64_t>(b) * a.Hkv + h;
-  for (int t = t0 + tid; t < min(t0 + kFinishTokens, ctx); t += kFinishThreads) {
+  for (int t = t0 + tid; t < min(t0 + kFinishTokens, plan.ctx); t += kFinishThreads) {
     if (t >= a.T) {
       spa_raise(SPA_DEVERR_BAD_INDEX);
       continue;
@@ -183,33 +250,26 @@ __global__ void __launch_bounds__(kFinishThreads) cache_decode_finish_kernel(con
 
 // ---------------------------------------------------------------------------
 // host planning
-constexpr int kCacheCtasPerSm = 4;
+constexpr int kWholeTiles = 24, kCtaTiles = 6;
 struct CachePlan {
   bool mma;
-  int heads, chunks, nsplit;
+  int heads, chunks, ctas, slots;
 };
-inline CachePlan cache_plan(int batch, int q_heads, int kv_heads, int head_dim, int max_candidates, int kv_dtype,
-                            bool mma) {
+inline CachePlan cache_plan(int batch, int q_heads, int kv_heads, int head_dim, int max_candidates, bool mma) {
   CachePlan p;
   const int group = q_heads / kv_heads;
   p.mma = mma;
-  const int warps = mma ? kI4Warps : kPlainWarps;
   p.heads = mma ? int4_mma_heads(head_dim, group) : kPlainHeads;
   p.chunks = (group + p.heads - 1) / p.heads;
-  (void)kv_dtype;
-  // the split count that ends first: waves of CTAs times a CTA's tiles (32 tokens a warp) and
-  // what a CTA costs besides them, about kCtaTiles tiles
-  constexpr int64_t kCtaTiles = 4;
-  const int64_t ctas = static_cast<int64_t>(batch) * kv_heads * p.chunks;
-  const int64_t slots = static_cast<int64_t>(device_sm_count()) * kCacheCtasPerSm;
+  const int64_t pairs = static_cast<int64_t>(batch) * kv_heads * p.chunks;
   const int64_t tiles = (max_candidates + 31) / 32 + 1;
-  int64_t best = 0;
-  p.nsplit = 1;
-  for (int64_t ns = 1; ns <= 64 && (ns == 1 || ns * warps < tiles + warps); ++ns) {
-    const int64_t each = (tiles + ns * warps - 1) / (ns * warps);
-    const int64_t cost = (ctas * ns + slots - 1) / slots * (each + kCtaTiles);
-    if (ns == 1 || cost < best) best = cost, p.nsplit = static_cast<int>(ns);
-  }
+  const int64_t room = static_cast<int64_t>(device_sm_count()) * (mma ? int4_mma_ctas(head_dim, p.heads) : 4);
+  const int64_t most = (pairs * tiles + kCtaTiles - 1) / kCtaTiles;
+  // One CTA per pair where a pair has little to share, where pairs alone fill the GPU several
+  // times over, or where the batch is longer than a CTA sums up.
+  const bool flat = tiles > kWholeTiles && pairs < 4 * room && batch <= kFlatBatch;
+  p.ctas = flat ? static_cast<int>(room < most ? room : most) : 0;
+  p.slots = static_cast<int>((flat ? p.ctas : pairs) + pairs);
   return p;
 }
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -219,7 +279,7 @@ struct CacheScratch {
 };
 inline CacheScratch cache_scratch(const CachePlan& p, int batch, int q_heads, int head_dim, int cap, bool weights) {
   CacheScratch s{};
-  const size_t parts = weights || p.nsplit > 1 ? static_cast<size_t>(batch) * q_heads * p.nsplit : 0;
+  const size_t parts = weights || p.ctas ? static_cast<size_t>(p.slots) * p.heads : 0;
   s.part_o = 0;
   s.part_lse = align256(parts * head_dim * sizeof(float));
   s.scores = s.part_lse + align256(parts * sizeof(float));
@@ -229,7 +289,7 @@ inline CacheScratch cache_scratch(const CachePlan& p, int batch, int q_heads, in
 
 template <typename T>
 int launch_cache_plain(const CacheDecodeArgs& a, cudaStream_t st) {
-  const dim3 grid(a.nsplit, a.Hkv * a.chunks, a.B);
+  const dim3 grid(a.ctas ? a.ctas : a.B * a.Hkv * a.chunks);
   const int e = (a.D + 31) / 32;
   if (e <= 1)
     cache_decode_plain_kernel<T, 1><<<grid, kPlainWarps * 32, 0, st>>>(a);
@@ -255,9 +315,9 @@ int cache_decode_impl(CacheDecodeArgs a, int kv_dtype, const spa_kv_layout* kv, 
   if ((a.selected && a.top_m <= 0) || (a.weights && (a.T <= 0 || a.selected))) return SPA_ERR_INVALID;
   a.group = a.Hq / a.Hkv;
   if (a.group > 256) return SPA_ERR_UNSUPPORTED;
-  const CachePlan p = cache_plan(a.B, a.Hq, a.Hkv, a.D, max_candidates, kv_dtype,
-                                 kv_dtype < 0 && int4_mma_serves(a.D, kv->total_rows));
-  if (static_cast<int64_t>(a.Hkv) * p.chunks > 65535) return SPA_ERR_UNSUPPORTED;
+  if (a.Hkv > 65535 || static_cast<int64_t>(a.B) * a.Hq > (1 << 28)) return SPA_ERR_UNSUPPORTED;
+  const CachePlan p =
+      cache_plan(a.B, a.Hq, a.Hkv, a.D, max_candidates, kv_dtype < 0 && int4_mma_serves(a.D, kv->total_rows));
   const CacheScratch s = cache_scratch(p, a.B, a.Hq, a.D, a.cap, a.weights != nullptr);
   if (s.total && (!workspace || workspace_bytes < s.total || reinterpret_cast<uintptr_t>(workspace) % 16))
     return SPA_ERR_WORKSPACE;
@@ -268,10 +328,10 @@ int cache_decode_impl(CacheDecodeArgs a, int kv_dtype, const spa_kv_layout* kv, 
   a.q_vec = reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
   a.heads = p.heads;
   a.chunks = p.chunks;
-  a.nsplit = p.nsplit;
+  a.ctas = p.ctas;
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   unsigned char* ws = static_cast<unsigned char*>(workspace);
-  const bool parts = a.weights || a.nsplit > 1;
+  const bool parts = a.weights || a.ctas;
   a.part_o = parts ? reinterpret_cast<float*>(ws + s.part_o) : nullptr;
   a.part_lse = parts ? reinterpret_cast<float*>(ws + s.part_lse) : nullptr;
   a.scores = a.weights ? reinterpret_cast<float*>(ws + s.scores) : nullptr;
@@ -289,8 +349,8 @@ int cache_decode_impl(CacheDecodeArgs a, int kv_dtype, const spa_kv_layout* kv, 
     rc = launch_cache_plain<__nv_bfloat16>(a, st);
   if (rc || !parts) return rc;
   const int span = a.local_window > 0 && a.local_window < a.cap ? a.local_window : a.cap;
-  const int blocks = a.group + (a.weights ? (span + kFinishTokens - 1) / kFinishTokens : 0);
-  SPA_CHECK_CUDA(launch_pdl(cache_decode_finish_kernel, dim3(blocks, a.Hkv, a.B), dim3(kFinishThreads), 0, st, true, a));
+  const int blocks = (a.group + kFinishHeads - 1) / kFinishHeads + (a.weights ? (span + kFinishTokens - 1) / kFinishTokens : 0);
+  SPA_CHECK_CUDA(launch_pdl(cache_decode_finish_kernel<32>, dim3(blocks, a.Hkv, a.B), dim3(kFinishThreads), 0, st, true, a));
   return SPA_OK;
 }
 
@@ -303,8 +363,8 @@ extern "C" size_t spa_cache_decode_workspace_size(int batch, int q_heads, int kv
     return 0;
   // the number of rows decides between the kernels, and it is not known here: the larger need
   size_t most = 0;
-  for (int mma = 0; mma < 2; ++mma) {
-    const spa::CachePlan p = spa::cache_plan(batch, q_heads, kv_heads, head_dim, max_candidates, kv_dtype, mma != 0);
+  for (int mma = 0; mma < (kv_dtype < 0 ? 2 : 1); ++mma) {
+    const spa::CachePlan p = spa::cache_plan(batch, q_heads, kv_heads, head_dim, max_candidates, mma != 0);
     const size_t need = spa::cache_scratch(p, batch, q_heads, head_dim, max_tokens, weights != 0).total;
     most = need > most ? need : most;
   }

@@ -20,16 +20,23 @@
 // (2 roundings of 2^-11 against the output's 2^-8), as two halves (22 bits) otherwise.
 //
 // What bounds it: HBM, 160 bytes a token and kv head at D = 128, if the instructions keep up:
-// at 6.5 TB/s an SM has 2.8 issue slots per value.  Each warp streams its own tiles of 32
-// tokens (5 KB) through a ring of cp.async stages in shared memory, without barriers between
-// warps, so pages of any size, order and alignment cost the same.
+// at 6.5 TB/s an SM has 2.8 issue slots per value, and a tile takes 2.6 a value.  Each warp
+// streams a stretch of tiles of 32 tokens (5 KB) through its own ring of cp.async stages in
+// shared memory, without barriers between warps, so pages of any size, order and alignment
+// cost the same.
 #pragma once
 
 #include "cache_args.cuh"
 
 namespace spa {
 
-constexpr int kI4Warps = 4, kI4Stages = 2, kI4Blocks = 4;
+template <int G, int NT>
+struct Int4Cfg {
+  // as many warps an SM as the registers allow (168, or 255 with the larger accumulators)
+  static constexpr bool kSmall = NT == 1 && G <= 4;
+  static constexpr int kWarps = kSmall ? 4 : 8, kCtas = kSmall ? 3 : 1;
+  static constexpr int kStages = 2;
+};
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -170,51 +177,73 @@ __device__ __forceinline__ void centre_zero(uint32_t& z, uint32_t& low, uint32_t
 // PREC 0: bf16 queries and outputs; 1: fp16 (probabilities in two halves); 2: fp32 (queries
 // in two halves as well).  NT: query heads served, in eights.
 template <int G, int NT, int PREC>
-__global__ void __launch_bounds__(kI4Warps * 32, NT == 1 && G <= 4 ? kI4Blocks : 2) int4_decode_mma_kernel(const CacheDecodeArgs a) {
+__global__ void __launch_bounds__(Int4Cfg<G, NT>::kWarps * 32, Int4Cfg<G, NT>::kCtas) int4_decode_mma_kernel(const CacheDecodeArgs a) {
   using S = Int4Tile<G>;
+  constexpr int W = Int4Cfg<G, NT>::kWarps, ST = Int4Cfg<G, NT>::kStages;
   constexpr int D = 32 * G, HN = 8 * NT;
   constexpr bool kCentreK = PREC == 2;
   constexpr float kSlack = 4.f, kUnit2 = 15.f - kSlack;
   constexpr float kUnitK = kCentreK ? 1.f : 16777216.f;
+  static_assert(NT * G <= W, "a warp prepares one group of query values");
   extern __shared__ __align__(128) unsigned char i4_smem[];
-  __shared__ unsigned s_live[kI4Warps][kI4Stages];
-  const int split = blockIdx.x, h = blockIdx.y / a.chunks, chunk = blockIdx.y % a.chunks, b = blockIdx.z;
+  __shared__ __align__(16) uint32_t s_q[PREC == 2 ? 2 : 1][NT * G][32][4];  // query fragments
+  __shared__ float s_big[NT * G][8], s_sum[NT * G][8], s_unit[HN];
+  __shared__ float s_f[HN][16];
+  __shared__ unsigned s_live[W][ST];
+  __shared__ int pre[kFlatBatch + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int head0 = chunk * HN, heads = min(HN, a.group - head0);
+  unsigned char* ring = i4_smem + warp * (ST * S::kStage);
+  pdl_trigger();
+  if (a.ctas) tiles_before<S::kTok>(a, pre);
+  Work work(a, pre);
+  Segment seg;
+#pragma unroll 1
+  while (work.next<S::kTok>(a, pre, seg)) {
+  const int b = seg.b, h = seg.h, head0 = seg.chunk * HN, heads = min(HN, a.group - head0);
   const int64_t q0 = static_cast<int64_t>(b) * a.Hq + h * a.group + head0;
-  unsigned char* ring = i4_smem + warp * (kI4Stages * S::kStage);
-
   const TilePlan plan = tile_plan<S::kTok>(a, b);
-  int t0, t1, w0, w1;
-  split_range(plan.n, split, a.nsplit, t0, t1);
-  split_range(t1 - t0, warp, kI4Warps, w0, w1);
-  w0 += t0, w1 += t0;  // this warp's tiles
 
-  // ---- a tile's rows, looked up one tile ahead of its loads.  Tiles that follow it in its page
-  // need no lookup: `run` of them start at row `flat`.
-  int next_tile = w0, next_row = -1, ahead = 0, run = 0, flat = 0;
-  const auto look_up = [&]() {
-    if (next_tile < w1)
-      next_row = static_cast<int>(
-          token_row(a, b, h, tile_token<S::kTok>(a, plan, b, next_tile, lane), plan.ctx, ahead));
+  int next_tile, end_tile;  // this warp's tiles, one stretch
+  split_range(seg.u1 - seg.u0, warp, W, next_tile, end_tile);
+  next_tile += seg.u0, end_tile += seg.u0;
+  const int first_tile = next_tile, n_tiles = end_tile - next_tile;
+
+  // ---- rows of the next tiles.  A tile's page is fetched one tile before its loads are issued.
+  // A full tile inside one page takes one look-up, good for the `run` full tiles that are left in
+  // the page, from row `flat` on; other tiles have a token, a page and a row a lane.
+  int token = -1, page = -1, page_off = 0, run = 0, flat = 0;
+  bool one_page = false;
+  const auto fetch = [&]() {
+    const int first = tile_token<S::kTok>(a, plan, b, next_tile, 0), last = tile_token<S::kTok>(a, plan, b, next_tile, S::kTok - 1);
+    one_page = false;
+    if (first >= 0 && last >= 0) {
+      page = token_page(a, b, first, page_off);
+      token = first;
+      one_page = page_off + S::kTok <= a.addr.page_size;
+    }
+    if (!one_page) {
+      token = tile_token<S::kTok>(a, plan, b, next_tile, lane);
+      page = token < 0 ? -1 : token_page(a, b, token, page_off);
+    }
   };
-  look_up();
+  if (next_tile < end_tile) fetch();
   const unsigned char* k_lane = static_cast<const unsigned char*>(a.k) + lane * 16;
   const unsigned char* v_lane = static_cast<const unsigned char*>(a.v) + lane * 16;
   const unsigned char* kz_lane = reinterpret_cast<const unsigned char*>(a.k_scales) + lane * S::kScaleChunk;
   const unsigned char* vz_lane = reinterpret_cast<const unsigned char*>(a.v_scales) + lane * S::kScaleChunk;
   const int put = S::at(lane / G, lane % G * 16);
   const auto issue = [&](int stage) {
-    if (next_tile < w1) {
+    if (next_tile < end_tile) {
       const uint32_t base = smem_u32(ring + stage * S::kStage);
+      constexpr int per = S::kScaleRow / S::kScaleChunk;
+      int row = -1;
       if (run == 0) {
-        const int first = __shfl_sync(0xffffffffu, next_row, 0);
-        if (__all_sync(0xffffffffu, first >= 0 && next_row == first + lane)) {
-          flat = first;
-          run = max(__shfl_sync(0xffffffffu, ahead, 0) / S::kTok, 1);
+        row = static_cast<int>(page_row(a, b, h, token, page, page_off));
+        if (one_page && row >= 0) {
+          flat = row;
+          run = min(a.addr.page_size - page_off, plan.ctx - token) / S::kTok;
         }
       }
-      constexpr int per = S::kScaleRow / S::kScaleChunk;
       if (run > 0) {
         // 32 rows on end: one address an array
         if (lane == 0) s_live[warp][stage] = 0xffffffffu;
@@ -239,7 +268,6 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 && G <= 4 ? kI4Blocks :
         flat += S::kTok;
         --run;
       } else {
-        const int row = next_row;
         const unsigned live = __ballot_sync(0xffffffffu, row >= 0);
         if (lane == 0) s_live[warp][stage] = live;
 #pragma unroll
@@ -262,59 +290,69 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 && G <= 4 ? kI4Blocks :
           cp_async<S::kScaleChunk>(dst + S::kScales, reinterpret_cast<const unsigned char*>(a.v_scales) + src, n);
         }
       }
-      ++next_tile;
-      if (run == 0) look_up();
+      if (++next_tile < end_tile && run == 0) fetch();
     }
     cp_async_commit();
   };
-#pragma unroll
-  for (int s = 0; s < kI4Stages - 1; ++s) issue(s);
+  issue(0);
 
-  // ---- the queries as B fragments.  A row is scaled by a power of two to a largest value in
-  // [2^9, 2^10): fp16 then holds 16-bit queries exactly, and group sums stay in range.
+  // ---- the queries as B fragments, a group of 32 values (of 8 heads) a warp.  A row is scaled
+  // by a power of two to a largest value in [2^9, 2^10): fp16 then holds 16-bit queries exactly,
+  // and group sums stay in range.
+  float x[8], big = 0.f;
+  if (warp < NT * G) {
+    const int head = warp / G * 8 + g;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+    if (head < heads) load8_any(a.q, a.dtype, (q0 + head) * D + 32 * (warp % G) + 8 * t, a.q_vec, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(x[i]));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    s_big[warp][g] = big;
+  }
+  __syncthreads();
+  if (warp < NT * G) {
+    const int n = warp / G;
+#pragma unroll
+    for (int j = 0; j < G; ++j) big = fmaxf(big, s_big[n * G + j][g]);
+    int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;  // floor(log2) of a normal number
+    e = big == 0.f || e == 128 ? 9 : min(max(e, -110), 120);
+    const float up = __uint_as_float(static_cast<uint32_t>(127 - e + 9) << 23);
+    s_unit[n * 8 + g] = __uint_as_float(static_cast<uint32_t>(127 + e - 9) << 23) * a.scale_log2;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += x[i] *= up;
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = !kCentreK && i & 1 ? 0.0625f : 1.f;
+      hi[i] = pack_h2(x[i] * f, x[i + 4] * f);
+      lo[i] = pack_h2(x[i] * f - half_lo(hi[i]), x[i + 4] * f - half_hi(hi[i]));
+    }
+    *reinterpret_cast<uint4*>(s_q[0][warp][lane]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if constexpr (PREC == 2) *reinterpret_cast<uint4*>(s_q[PREC == 2][warp][lane]) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    s_sum[warp][g] = sum;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int s = 1; s < ST - 1; ++s) issue(s);
   uint32_t qb[NT][G][2][2], ql[NT][G][2][2], qz[NT][2];
   float q_unit[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int head = n * 8 + g;
-    float x[G][8], big = 0.f;
 #pragma unroll
     for (int j = 0; j < G; ++j) {
-      if (head < heads)
-        load8_any(a.q, a.dtype, (q0 + head) * D + 32 * j + 8 * t, a.q_vec, x[j]);
-      else
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(x[j][i]));
+      *reinterpret_cast<uint4*>(&qb[n][j][0][0]) = *reinterpret_cast<const uint4*>(s_q[0][n * G + j][lane]);
+      if constexpr (PREC == 2)
+        *reinterpret_cast<uint4*>(&ql[n][j][0][0]) = *reinterpret_cast<const uint4*>(s_q[PREC == 2][n * G + j][lane]);
     }
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-    int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;  // floor(log2) of a normal number
-    e = big == 0.f || e == 128 ? 9 : min(max(e, -110), 120);
-    const float up = __uint_as_float(static_cast<uint32_t>(127 - e + 9) << 23);
-    const float down = __uint_as_float(static_cast<uint32_t>(127 + e - 9) << 23) * a.scale_log2;
-    q_unit[n][0] = __shfl_sync(0xffffffffu, down, 8 * t);
-    q_unit[n][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
-    float z0 = 0.f, z1 = 0.f;  // sums of groups 2t and 2t + 1
-#pragma unroll
-    for (int j = 0; j < G; ++j) {
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum += x[j][i] *= up;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float f = !kCentreK && i & 1 ? 0.0625f : 1.f;
-        const float lo = x[j][i] * f, hi = x[j][i + 4] * f;
-        qb[n][j][i >> 1][i & 1] = pack_h2(lo, hi);
-        if constexpr (PREC == 2)
-          ql[n][j][i >> 1][i & 1] = pack_h2(lo - half_lo(qb[n][j][i >> 1][i & 1]), hi - half_hi(qb[n][j][i >> 1][i & 1]));
-      }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      if (j == 2 * t) z0 = sum;
-      if (j == 2 * t + 1) z1 = sum;
-    }
+    q_unit[n][0] = s_unit[n * 8 + 2 * t];
+    q_unit[n][1] = s_unit[n * 8 + 2 * t + 1];
+    // sums of groups 2t and 2t + 1
+    const float z0 = 2 * t < G ? s_sum[n * G + 2 * t][g] : 0.f, z1 = 2 * t + 1 < G ? s_sum[n * G + 2 * t + 1][g] : 0.f;
     qz[n][0] = pack_h2(z0, z1);
     qz[n][1] = pack_h2(z0 - half_lo(qz[n][0]), z1 - half_hi(qz[n][0]));
   }
@@ -348,10 +386,10 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 && G <= 4 ? kI4Blocks :
 
   int stage = 0;
 #pragma unroll 1
-  for (int tile = w0; tile < w1; ++tile) {
-    cp_async_wait<kI4Stages - 2>();
+  for (int done = 0; done < n_tiles; ++done) {
+    cp_async_wait<ST - 2>();
     __syncwarp();
-    issue(stage == 0 ? kI4Stages - 1 : stage - 1);  // the stage that the previous tile left
+    issue(stage == 0 ? ST - 1 : stage - 1);  // the stage that the previous tile left
     const unsigned char* ks = ring + stage * S::kStage;
     const unsigned char* vs = ks + S::kCodes;
     const unsigned char* ksc = ks + 2 * S::kCodes;
@@ -439,7 +477,7 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 && G <= 4 ? kI4Blocks :
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int tok = plan.seg + tile * S::kTok + hh * 16 + g + (e < 2 ? 0 : 8), head = n * 8 + 2 * t + (e & 1);
+            const int tok = plan.seg + (first_tile + done) * S::kTok + hh * 16 + g + (e < 2 ? 0 : 8), head = n * 8 + 2 * t + (e & 1);
             if (tok >= plan.lo && tok < plan.ctx && head < heads)
               a.scores[((static_cast<int64_t>(b) * a.Hkv + h) * a.cap + tok) * a.group + head0 + head] = sc[hh][n][e] * q_unit[n][e & 1];
           }
@@ -582,7 +620,7 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 && G <= 4 ? kI4Blocks :
       };
       for_each_index(group, std::make_integer_sequence<int, G>{});
     }
-    stage = stage == kI4Stages - 1 ? 0 : stage + 1;
+    stage = stage == ST - 1 ? 0 : stage + 1;
   }
 
   // ---- merge the warps (the ring is free once every copy has landed)
@@ -611,31 +649,47 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 && G <= 4 ? kI4Blocks :
     }
   }
   __syncthreads();
-  for (int i = tid; i < heads * D; i += kI4Warps * 32) {
-    const int n = i / D, d = i % D;
-    const float* row = buf + n * kLd;
-    float M = -INFINITY, W = 0.f, O = 0.f;
+  const bool partial = a.weights || !seg.whole;
+  if (tid < HN * 16) {  // a head's warps side by side: their shares of the whole
+    const int n = tid >> 4, w = tid & 15;
+    const float* row = buf + (w * HN + n) * kLd + D;
+    const float mw = w < W ? row[0] : -INFINITY, lw = w < W ? row[1] : 0.f;
+    float M = mw;
 #pragma unroll
-    for (int w = 0; w < kI4Warps; ++w) M = fmaxf(M, row[w * HN * kLd + D]);
+    for (int off = 1; off < 16; off <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    const float f = mw == -INFINITY ? 0.f : fast_exp2(mw - M);
+    float sum = lw * f;
 #pragma unroll
-    for (int w = 0; w < kI4Warps; ++w) {
-      const float mw = row[w * HN * kLd + D], f = mw == -INFINITY ? 0.f : fast_exp2(mw - M);
-      W = fmaf(row[w * HN * kLd + D + 1], f, W);
-      O = fmaf(row[w * HN * kLd + d], f, O);
+    for (int off = 1; off < 16; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    // no token at all (sum 0): zeros
+    s_f[n][w] = sum == 0.f ? 0.f : f / sum;
+    if (partial && w == 0 && n < heads)
+      a.part_lse[static_cast<int64_t>(seg.slot) * HN + n] = sum == 0.f ? -INFINITY : M + log2f(sum);
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int i = tid; i < heads * (D / 4); i += W * 32) {
+    const int n = i / (D / 4), d = i % (D / 4) * 4;
+    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int w = 0; w < W; ++w) {
+      const float f = s_f[n][w];
+      const float4 v = *reinterpret_cast<const float4*>(buf + (w * HN + n) * kLd + d);
+      r.x = fmaf(v.x, f, r.x), r.y = fmaf(v.y, f, r.y), r.z = fmaf(v.z, f, r.z), r.w = fmaf(v.w, f, r.w);
     }
-    const float out = W == 0.f ? 0.f : O / W;
-    if (a.part_o) {
-      a.part_o[((q0 + n) * a.nsplit + split) * D + d] = out;
-      if (d == 0) a.part_lse[(q0 + n) * a.nsplit + split] = W == 0.f ? -INFINITY : M + log2f(W);
-    } else {
-      store_any(a.out, a.dtype, (q0 + n) * D + d, out);
-    }
+    if (partial)
+      *reinterpret_cast<float4*>(a.part_o + (static_cast<int64_t>(seg.slot) * HN + n) * D + d) = r;
+    else
+      store4_any(a.out, a.dtype, (q0 + n) * D + d, r);
+  }
+  __syncthreads();  // the next segment's loads reuse the buffer
   }
 }
 
 template <int G, int NT>
 constexpr int int4_smem_bytes() {
-  constexpr int ring = kI4Warps * kI4Stages * Int4Tile<G>::kStage, merge = kI4Warps * 8 * NT * (32 * G + 4) * 4;
+  constexpr int W = Int4Cfg<G, NT>::kWarps, ring = W * Int4Cfg<G, NT>::kStages * Int4Tile<G>::kStage;
+  constexpr int merge = W * 8 * NT * (32 * G + 4) * 4;
   return ring > merge ? ring : merge;
 }
 template <int G, int NT, int PREC>
@@ -643,7 +697,7 @@ int launch_int4_mma(const CacheDecodeArgs& a, cudaStream_t st) {
   auto kern = int4_decode_mma_kernel<G, NT, PREC>;
   constexpr int smem = int4_smem_bytes<G, NT>();
   SPA_CHECK_CUDA(spa_set_smem_once(kern, smem));
-  kern<<<dim3(a.nsplit, a.Hkv * a.chunks, a.B), kI4Warps * 32, smem, st>>>(a);
+  kern<<<a.ctas ? a.ctas : a.B * a.Hkv * a.chunks, Int4Cfg<G, NT>::kWarps * 32, smem, st>>>(a);
   SPA_CHECK_CUDA(cudaGetLastError());
   return SPA_OK;
 }
@@ -656,6 +710,7 @@ int launch_int4_prec(const CacheDecodeArgs& a, cudaStream_t st) {
 // Query heads a CTA serves: one matrix column block of 8, or two where the registers allow
 // (not at head_dim 256), so that up to 16 heads share one read of K and V.
 inline int int4_mma_heads(int head_dim, int group) { return group > 8 && head_dim < 256 ? 16 : 8; }
+inline int int4_mma_ctas(int head_dim, int heads) { return heads == 8 && head_dim <= 128 ? 3 : 1; }
 inline bool int4_mma_serves(int head_dim, int64_t total_rows) {
   return (head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 256) &&
          total_rows < (1ll << 31);  // rows travel between lanes as 32-bit numbers
