@@ -108,13 +108,13 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(const float*
 
 // In-place compaction.  Of one (sequence, kv head) row j <- row keep[j] with keep ascending,
 // so no source lies before its destination.  A cluster of CTAs takes the rows of one pool in
-// order, a chunk at a time: every thread loads its 16-byte units of the chunk, and they are
-// stored once the whole cluster has loaded.  The next chunk's sources lie behind every row
-// stored so far, so its loads are in flight meanwhile.
+// order, a chunk at a time: every thread loads its units (16 bytes where rows allow) of the
+// chunk, and they are stored once the whole cluster has loaded.  The next chunk's sources lie
+// behind every row stored so far, so its loads are in flight meanwhile, and the rows of the
+// chunk after that (keep, then the page table) are being looked up, once a row.
 //
 // Bound by HBM (each kept row read and written once).  One CTA a pool and pair leaves that to
-// the latency of its chunks: 64 pairs, 8192 of 32768 rows of 256 bytes took 777 us in this
-// scheme with single CTAs.
+// the latency of its chunks: 64 pairs, 8192 of 32768 rows of 256 bytes took 777 us that way.
 constexpr int kMaxPools = 8;
 struct CompactArgs {
   unsigned char* pool[kMaxPools];
@@ -130,9 +130,8 @@ struct CompactArgs {
 
 constexpr int kCompactThreads = 256, kCompactUnroll = 4;
 
-// Byte address of token t's row, or nullptr (with the error word set) where it has no page.
-__device__ __forceinline__ unsigned char* compact_row(const CompactArgs& a, unsigned char* pool, int bytes, int b,
-                                                      int h, int t) {
+// Row of token t, or -1 (with the error word set) where it has no page.
+__device__ __forceinline__ int64_t compact_row(const CompactArgs& a, int b, int h, int t) {
   int lp = static_cast<int>(__umulhi(static_cast<uint32_t>(t), a.page_inv)), off = t - lp * a.addr.page_size;
   if (off >= a.addr.page_size) ++lp, off -= a.addr.page_size;
   const int64_t pg = a.addr.page_of(b, lp);
@@ -140,70 +139,91 @@ __device__ __forceinline__ unsigned char* compact_row(const CompactArgs& a, unsi
       b * a.addr.batch_stride_rows + pg * a.addr.page_stride_rows + h * a.addr.head_stride_rows + off;
   if (pg < 0 || row < 0 || row >= a.addr.total_rows) {
     spa_raise(SPA_DEVERR_BAD_PAGE);
-    return nullptr;
+    return -1;
   }
-  return pool + row * bytes;
+  return row;
 }
 
-// rows: of the pair; per: units a row; rank, ranks: of the CTA in its cluster.  at(j): the
-// addresses of source and destination row j, both null to leave the row out.
+// A chunk of a CTA: the fewer of 256 rows and what its threads hold in kCompactUnroll units each.
+__host__ __device__ inline int compact_chunk_rows(int per) {
+  const int rows = kCompactThreads * kCompactUnroll / per;
+  return rows < 1 ? 1 : rows < kCompactThreads ? rows : kCompactThreads;
+}
+
+// rows: of the pair; per: units a row; rank, ranks: of the CTA in its cluster; slot: 4 tables of
+// a chunk's (source, destination) rows, so that a thread may be a chunk ahead of another.
+// at(j, from, to): rows of entry j of the list, to < 0 to leave it out.
 template <typename U, typename At>
-__device__ __forceinline__ void compact_rows(int rows, int per, int rank, int ranks, At at) {
-  constexpr int kSpan = kCompactThreads * kCompactUnroll;
-  const uint32_t units = static_cast<uint32_t>(rows) * per;  // host: fits
-  const uint32_t step = static_cast<uint32_t>(ranks) * kSpan;
-  U v[2][kCompactUnroll] = {};
-  U* dst[2][kCompactUnroll];
-  const auto load = [&](uint32_t base, int k) {
+__device__ __forceinline__ void compact_rows(U* pool, int rows, int per, int rank, int ranks,
+                                             longlong2 (*slot)[kCompactThreads], At at) {
+  const int chunk = compact_chunk_rows(per), chunks = (rows + chunk * ranks - 1) / (chunk * ranks);
+  int row_of[kCompactUnroll], off_of[kCompactUnroll];  // of this thread's units, in every chunk
 #pragma unroll
-    for (int u = 0; u < kCompactUnroll; ++u) {
-      const uint32_t i = base + rank * kSpan + u * kCompactThreads + threadIdx.x;
-      dst[k][u] = nullptr;
-      if (i < units) {
-        const uint32_t j = i / per, off = i - j * per;
-        unsigned char *from, *to;
-        at(static_cast<int>(j), from, to);
-        if (to) {
-          dst[k][u] = reinterpret_cast<U*>(to) + off;
-          v[k][u] = reinterpret_cast<const U*>(from)[off];
-        }
-      }
+  for (int u = 0; u < kCompactUnroll; ++u) {
+    const int i = threadIdx.x + u * kCompactThreads;
+    row_of[u] = i / per;
+    off_of[u] = i - row_of[u] * per;
+    if (row_of[u] >= chunk) row_of[u] = -1;
+  }
+  const auto look_up = [&](int c) {
+    if (static_cast<int>(threadIdx.x) < chunk) {
+      const int j = (c * ranks + rank) * chunk + threadIdx.x;
+      int64_t from = -1, to = -1;
+      if (c < chunks && j < rows) at(j, from, to);
+      slot[c & 3][threadIdx.x] = make_longlong2(from, to);
     }
   };
-  const auto store = [&](int k) {
+  U v[2][kCompactUnroll] = {};
+  const auto load = [&](int c, int k) {
 #pragma unroll
     for (int u = 0; u < kCompactUnroll; ++u)
-      if (dst[k][u]) *dst[k][u] = v[k][u];
+      if (row_of[u] >= 0) {
+        const longlong2 r = slot[c & 3][row_of[u]];
+        if (r.y >= 0) v[k][u] = pool[r.x * per + off_of[u]];
+      }
   };
-  // the loads have returned before the cluster is told so
+  const auto store = [&](int c, int k) {
+#pragma unroll
+    for (int u = 0; u < kCompactUnroll; ++u)
+      if (row_of[u] >= 0) {
+        const longlong2 r = slot[c & 3][row_of[u]];
+        if (r.y >= 0) pool[r.y * per + off_of[u]] = v[k][u];
+      }
+  };
+  // The loads have returned before the cluster is told that they have: that orders them before
+  // the others' stores, so the arrival needs no fence (which would wait for the last chunk's
+  // stores).  The CTA barrier after the wait orders the tables.
   const auto arrive = [&](int k) {
 #pragma unroll
     for (int u = 0; u < kCompactUnroll; ++u) {
-      const unsigned char* p = reinterpret_cast<const unsigned char*>(&v[k][u]);
       if constexpr (sizeof(U) >= 4) {
 #pragma unroll
-        for (int w = 0; w < static_cast<int>(sizeof(U)) / 4; ++w) asm volatile("" ::"r"(reinterpret_cast<const uint32_t*>(p)[w]));
+        for (int w = 0; w < static_cast<int>(sizeof(U)) / 4; ++w)
+          asm volatile("" ::"r"(reinterpret_cast<const uint32_t*>(&v[k][u])[w]) : "memory");
       } else {
-        asm volatile("" ::"r"(static_cast<uint32_t>(*reinterpret_cast<const U*>(p))));
+        asm volatile("" ::"r"(static_cast<uint32_t>(v[k][u])) : "memory");
       }
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    cluster_arrive_relaxed();
   };
-  const auto wait = [] { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); };
+  look_up(0);
+  look_up(1);
+  __syncthreads();
   load(0, 0);
-  for (uint32_t base = 0; base < units; base += 2 * step) {
-    arrive(0);
-    load(base + step, 1);
-    wait();
-    store(0);
-    arrive(1);
-    if (base + 2 * step < units) load(base + 2 * step, 0);
-    wait();
-    store(1);
+  for (int c = 0; c < chunks; c += 2) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      look_up(c + k + 2);
+      arrive(k);
+      if (c + k + 1 < chunks) load(c + k + 1, 1 - k);
+      cluster_wait();
+      __syncthreads();
+      if (c + k < chunks) store(c + k, k);
+    }
   }
 }
 
-__global__ void __launch_bounds__(kCompactThreads) compact_kernel(const CompactArgs a) {
+__global__ void __launch_bounds__(kCompactThreads, 4) compact_kernel(const CompactArgs a) {
   uint32_t rank, ranks;
   asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
   asm volatile("mov.u32 %0, %cluster_nctarank;" : "=r"(ranks));
@@ -240,29 +260,29 @@ __global__ void __launch_bounds__(kCompactThreads) compact_kernel(const CompactA
     if (threadIdx.x == 0) spa_raise(SPA_DEVERR_BAD_INDEX);
     return;
   }
+  __shared__ longlong2 s_rows[4][kCompactThreads];
   if (which < a.n_pools) {
     unsigned char* pool = a.pool[which];
     const int bytes = a.row_bytes[which];
     // a row whose source or destination has no page is left out whole
-    const auto at = [&](int j, unsigned char*& from, unsigned char*& to) {
+    const auto at = [&](int j, int64_t& from, int64_t& to) {
       const int k = keep[j];
-      from = to = nullptr;
       if (k == j) return;
-      from = compact_row(a, pool, bytes, b, h, k);
-      if (from) to = compact_row(a, pool, bytes, b, h, j);
+      from = compact_row(a, b, h, k);
+      if (from >= 0) to = compact_row(a, b, h, j);
     };
     switch (a.unit[which]) {
-      case 16: compact_rows<uint4>(n, bytes / 16, rank, ranks, at); break;
-      case 8: compact_rows<uint2>(n, bytes / 8, rank, ranks, at); break;
-      case 4: compact_rows<uint32_t>(n, bytes / 4, rank, ranks, at); break;
-      case 2: compact_rows<uint16_t>(n, bytes / 2, rank, ranks, at); break;
-      default: compact_rows<unsigned char>(n, bytes, rank, ranks, at); break;
+      case 16: compact_rows(reinterpret_cast<uint4*>(pool), n, bytes / 16, rank, ranks, s_rows, at); break;
+      case 8: compact_rows(reinterpret_cast<uint2*>(pool), n, bytes / 8, rank, ranks, s_rows, at); break;
+      case 4: compact_rows(reinterpret_cast<uint32_t*>(pool), n, bytes / 4, rank, ranks, s_rows, at); break;
+      case 2: compact_rows(reinterpret_cast<uint16_t*>(pool), n, bytes / 2, rank, ranks, s_rows, at); break;
+      default: compact_rows(pool, n, bytes, rank, ranks, s_rows, at); break;
     }
   } else if (a.weights) {
     float* w = a.weights + bh * a.T;
-    compact_rows<float>(n, 1, rank, ranks, [&](int j, unsigned char*& from, unsigned char*& to) {
-      from = reinterpret_cast<unsigned char*>(w + keep[j]);
-      to = reinterpret_cast<unsigned char*>(w + j);
+    compact_rows(reinterpret_cast<uint32_t*>(w), n, 1, rank, ranks, s_rows, [&](int j, int64_t& from, int64_t& to) {
+      from = keep[j];
+      to = j;
     });
     // the sources behind row n have all been loaded (an empty list had no chunk to wait for,
     // and no sources)
@@ -307,15 +327,15 @@ extern "C" int spa_compact_tokens(const spa_kv_layout* kv, int n_pools, void* co
   a.budget = budget;
   a.weights = weights;
   a.T = weight_tokens;
-  // CTAs a cluster: as many as have a chunk of the largest pool's rows, up to the portable 8
-  int64_t units = 1;
+  // CTAs a cluster: as many as have a chunk of some pool's rows, up to the portable 8
+  int64_t most = weights ? (budget + spa::kCompactThreads - 1) / spa::kCompactThreads : 1;
   for (int i = 0; i < n_pools; ++i) {
-    const int64_t u = static_cast<int64_t>(budget) * (row_bytes[i] / a.unit[i]);
-    if (u >> 31) return SPA_ERR_UNSUPPORTED;
-    units = u > units ? u : units;
+    const int per = row_bytes[i] / a.unit[i];
+    if (per > spa::kCompactThreads * spa::kCompactUnroll) return SPA_ERR_UNSUPPORTED;
+    const int64_t chunks = (budget + spa::compact_chunk_rows(per) - 1) / spa::compact_chunk_rows(per);
+    most = chunks > most ? chunks : most;
   }
-  const int64_t spans = (units + spa::kCompactThreads * spa::kCompactUnroll - 1) / (spa::kCompactThreads * spa::kCompactUnroll);
-  const int ranks = spans >= 8 ? 8 : spans >= 4 ? 4 : spans >= 2 ? 2 : 1;
+  const int ranks = most >= 8 ? 8 : most >= 4 ? 4 : most >= 2 ? 2 : 1;
   SPA_CHECK_CUDA(spa::launch_ex(spa::compact_kernel, dim3((n_pools + (weights ? 1 : 0)) * ranks, kv_heads, batch),
                                 dim3(spa::kCompactThreads), 0, reinterpret_cast<cudaStream_t>(stream), false, ranks, a));
   return SPA_OK;

@@ -22,25 +22,6 @@ namespace spa {
 
 constexpr int kInt4Group = 32;
 
-// Four consecutive values of a row as fp32; `vec` when the address allows one wide load.
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, bool vec, float (&x)[4]) {
-  if (vec) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(p);
-      x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-    } else {
-      const uint2 v = *reinterpret_cast<const uint2*>(p);
-      const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(e[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(p[i]);
-  }
-}
-
 struct Int4Rows {
   uint8_t* codes[2];  // K, V
   __half* scales[2];
@@ -62,89 +43,120 @@ __device__ __forceinline__ int64_t int4_row(const Int4Rows& a, int b, int h, int
   return row;
 }
 
-// Both kernels: a warp has one (sequence, kv head) and, of its rows, a stretch of kInt4Stretch;
-// eight lanes hold a group, four values each, so a warp covers 4 groups at once (a whole row of
-// head_dim 128, two rows of 64).  Grid (B * Hkv, K or V, stretches): no index is divided.
-// Bound by HBM (a row's 2 D bytes against its 5/8 D at 16 bits), reached by kInt4Flight steps'
-// loads in flight a lane.
-constexpr int kInt4Warps = 4, kInt4Stretch = 32, kInt4Flight = 4;
+// Both kernels: a warp has a stretch of 32 rows of one (sequence, kv head) and takes 32 / G of
+// them at a time.  Grid (B * Hkv, K or V, stretches): no index is divided but by G.  Codes
+// change places in shared memory (a lane has a group's 8 words, a row's 16 bytes hold words of
+// all groups), so that they move in 16-byte pieces.
+//
+// Bound by HBM (a row's 2 D bytes against its 5/8 D at 16 bits) as long as a value costs few
+// instructions: 9 here to quantise one; with a group spread over 8 lanes and a division a value
+// it was 63.
+constexpr int kInt4Warps = 4, kInt4Stretch = 32;
 
-struct Int4Lane {
-  int g, j0;  // the lane's place in its eight, and which eight of the warp it is in
-  __device__ __forceinline__ Int4Lane() : g(threadIdx.x & 7), j0((threadIdx.x & 31) >> 3) {}
-};
+// 32 consecutive values of a row as fp32; `vec` when 16-byte loads are allowed.
+template <typename T>
+__device__ __forceinline__ void load_group(const T* p, bool vec, float (&x)[32]) {
+  if (!vec) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = to_f32<T>(p[i]);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(x + 4 * i) = reinterpret_cast<const float4*>(p)[i];
+  } else {
+    uint4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+    const T* e = reinterpret_cast<const T*>(v);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = to_f32<T>(e[i]);
+  }
+}
+
+// A group's 8 words of 4 codes, its scale and zero.
+__device__ __forceinline__ void quantise_group(const float (&x)[32], uint32_t (&word)[8], __half& s, __half& z) {
+  float lo = x[0], hi = x[0], odd = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    lo = fminf(lo, x[i]);
+    hi = fmaxf(hi, x[i]);
+    odd = fmaf(x[i], 0.f, odd);  // NaN for a NaN or an infinity
+  }
+  s = __float2half_rn(fminf(__fdiv_rn(__fsub_rn(hi, lo), 15.f), 65504.f));
+  z = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
+  const bool bad = odd != 0.f;
+  const float sf = __half2float(s), zf = __half2float(z);
+  if (bad) s = z = __ushort_as_half(0x7fff);
+  const bool none = bad || !(sf > 0.f);
+  // rint((x - z) / s) by the clamped product with 1 / (15 s): within 4e-6 of the quotient, so
+  // where the product is further than that from a half it rounds to the same code.  Adding
+  // 1.5 2^23 rounds to the integer, ties to even.
+  constexpr float kMagic = 12582912.f;
+  const float inv = none ? 0.f : 1.f / (15.f * sf);
+  float off = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    float n[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float q = __saturatef(__fsub_rn(x[4 * w + e], zf) * inv);
+      n[e] = fmaf(q, 15.f, kMagic) - kMagic;
+      off = fmaxf(off, fabsf(fmaf(q, 15.f, -n[e])));
+    }
+    word[w] = static_cast<uint32_t>(fmaf(n[3], 4096.f, fmaf(n[2], 256.f, fmaf(n[1], 16.f, n[0]))));
+  }
+  if (off > 0.49999f && !none) {  // some value next to a half: the division decides
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      word[w] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float n = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[4 * w + e], zf), sf)), 0.f), 15.f);
+        word[w] |= static_cast<uint32_t>(n) << (4 * e);
+      }
+    }
+  }
+  if (none) {
+#pragma unroll
+    for (int w = 0; w < 8; ++w) word[w] = 0;
+  }
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kInt4Warps * 32) int4_append_kernel(const Int4Rows a, const T* __restrict__ k_new,
                                                                       const T* __restrict__ v_new, int64_t sb,
                                                                       int64_t sh, int64_t st, int vec) {
-  const Int4Lane ln;
-  const int which = blockIdx.y, warp = threadIdx.x >> 5, b = blockIdx.x / a.H, h = blockIdx.x - b * a.H;
+  __shared__ __align__(16) uint16_t s_words[kInt4Warps][256];
+  const int which = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H;
   const int len = a.lens ? min(a.lens[b], a.T) : a.T;
   const int t0 = (blockIdx.z * kInt4Warps + warp) * kInt4Stretch, t1 = min(t0 + kInt4Stretch, len);
   if (t0 >= t1) return;
   const T* src = (which ? v_new : k_new) + b * sb + h * sh;
-  uint16_t* codes = reinterpret_cast<uint16_t*>(which ? a.codes[1] : a.codes[0]);
+  uint8_t* codes = which ? a.codes[1] : a.codes[0];
   __half* scales = which ? a.scales[1] : a.scales[0];
-  // the stretch's rows, one a lane
-  const int64_t my_row = t0 + (threadIdx.x & 31) < t1 ? int4_row(a, b, h, t0 + (threadIdx.x & 31), true) : -1;
-  // steps: groups of the stretch in order, four (a lane's every fourth) at a time
-  const int steps = ((t1 - t0) * a.G + 3) >> 2;
-  int t = t0, j = ln.j0;  // this lane's row and group
-  while (j >= a.G) j -= a.G, ++t;
-  for (int s0 = 0; s0 < steps; s0 += kInt4Flight) {
-    float x[kInt4Flight][4];
-    int tt[kInt4Flight], jj[kInt4Flight];
+  const int64_t my_row = t0 + lane < t1 ? int4_row(a, b, h, t0 + lane, true) : -1;
+  // this lane's row among the step's, and its group (its 16-byte piece when storing)
+  const int rows = 32 / a.G, r = lane / a.G, j = lane - r * a.G;
+  uint16_t* words = s_words[warp];
+  for (int base = 0; base < t1 - t0; base += rows) {
+    const int i = base + r;
+    const bool in = r < rows && t0 + i < t1;
+    const int64_t row = __shfl_sync(0xffffffffu, my_row, in ? i : 0);
+    if (in && row >= 0) {
+      float x[32];
+      load_group<T>(src + (t0 + i) * st + j * kInt4Group, vec, x);
+      uint32_t word[8];
+      __half s, z;
+      quantise_group(x, word, s, z);
 #pragma unroll
-    for (int i = 0; i < kInt4Flight; ++i) {
-      tt[i] = t;
-      jj[i] = j;
-      if (t < t1)
-        load4<T>(src + t * st + j * kInt4Group + ln.g * 4, vec, x[i]);
-      else
-        x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
-      j += 4;
-      while (j >= a.G) j -= a.G, ++t;
+      for (int g = 0; g < 8; ++g) words[r * a.G * 8 + g * a.G + j] = static_cast<uint16_t>(word[g]);
+      scales[row * 2 * a.G + j] = s;
+      scales[row * 2 * a.G + a.G + j] = z;
     }
-#pragma unroll
-    for (int i = 0; i < kInt4Flight; ++i) {
-      const int64_t row = __shfl_sync(0xffffffffu, my_row, tt[i] - t0 < 31 ? tt[i] - t0 : 31);
-      float lo = fminf(fminf(x[i][0], x[i][1]), fminf(x[i][2], x[i][3]));
-      float hi = fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3]));
-      // x - x is NaN for a NaN or an infinity, 0 otherwise
-      float odd = (x[i][0] - x[i][0]) + (x[i][1] - x[i][1]) + (x[i][2] - x[i][2]) + (x[i][3] - x[i][3]);
-#pragma unroll
-      for (int off = 1; off < 8; off <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-        odd += __shfl_xor_sync(0xffffffffu, odd, off);
-      }
-      const bool bad = odd != 0.f;
-      __half s = __float2half_rn(fminf(__fdiv_rn(__fsub_rn(hi, lo), 15.f), 65504.f));
-      __half z = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
-      const float sf = __half2float(s), zf = __half2float(z);
-      uint32_t word = 0;
-      if (!bad && sf > 0.f) {
-        // rint((x - z) / s): the quotient by a reciprocal is within 2^-21 of it (three roundings,
-        // quotients of this range below 2^4 + 2), so only near a half the division itself decides
-        const float inv = __frcp_rn(sf);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float d = __fsub_rn(x[i][e], zf);
-          float n = d * inv;
-          const float frac = n - floorf(n);
-          if (fabsf(frac - 0.5f) < 1e-4f) n = __fdiv_rn(d, sf);
-          word |= static_cast<uint32_t>(fminf(fmaxf(rintf(n), 0.f), 15.f)) << (4 * e);
-        }
-      }
-      if (bad) s = z = __ushort_as_half(0x7fff);
-      if (tt[i] < t1 && row >= 0) {
-        codes[row * (a.G * 8) + ln.g * a.G + jj[i]] = static_cast<uint16_t>(word);
-        __half* sc = scales + row * 2 * a.G + jj[i];
-        if (ln.g == 0) sc[0] = s;
-        if (ln.g == 1) sc[a.G] = z;
-      }
-    }
+    __syncwarp();
+    if (in && row >= 0)
+      *reinterpret_cast<uint4*>(codes + row * (a.G * 16) + j * 16) = *reinterpret_cast<const uint4*>(words + lane * 8);
+    __syncwarp();
   }
 }
 
@@ -152,50 +164,55 @@ __global__ void __launch_bounds__(kInt4Warps * 32) int4_append_kernel(const Int4
 template <typename T>
 __global__ void __launch_bounds__(kInt4Warps * 32) int4_read_kernel(const Int4Rows a, T* __restrict__ k_out,
                                                                     T* __restrict__ v_out) {
-  const Int4Lane ln;
-  const int which = blockIdx.y, warp = threadIdx.x >> 5, b = blockIdx.x / a.H, h = blockIdx.x - b * a.H;
+  __shared__ __align__(16) uint16_t s_words[kInt4Warps][256];
+  __shared__ float2 s_scale[kInt4Warps][32];
+  const int which = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H;
   const int len = a.lens ? min(a.lens[b], a.T) : a.T;
   const int t0 = (blockIdx.z * kInt4Warps + warp) * kInt4Stretch, t1 = min(t0 + kInt4Stretch, a.T);
   if (t0 >= t1) return;
-  const uint16_t* codes = reinterpret_cast<const uint16_t*>(which ? a.codes[1] : a.codes[0]);
+  const uint8_t* codes = which ? a.codes[1] : a.codes[0];
   const __half* scales = which ? a.scales[1] : a.scales[0];
   T* dst = (which ? v_out : k_out) + static_cast<int64_t>(blockIdx.x) * a.T * (a.G * kInt4Group);
-  const int64_t my_row = t0 + (threadIdx.x & 31) < min(t1, len) ? int4_row(a, b, h, t0 + (threadIdx.x & 31), true) : -1;
-  const int steps = ((t1 - t0) * a.G + 3) >> 2;
-  int t = t0, j = ln.j0;
-  while (j >= a.G) j -= a.G, ++t;
-  for (int s0 = 0; s0 < steps; s0 += kInt4Flight) {
-    uint32_t word[kInt4Flight];
-    float s[kInt4Flight], z[kInt4Flight];
-    int tt[kInt4Flight], jj[kInt4Flight];
+  const int64_t my_row = t0 + lane < min(t1, len) ? int4_row(a, b, h, t0 + lane, true) : -1;
+  const int rows = 32 / a.G, r = lane / a.G, j = lane - r * a.G;
+  uint16_t* words = s_words[warp];
+  for (int base = 0; base < t1 - t0; base += rows) {
+    const int i = base + r;
+    const bool in = r < rows && t0 + i < t1;
+    const int64_t row = __shfl_sync(0xffffffffu, my_row, in ? i : 0);
+    uint4 piece = make_uint4(0, 0, 0, 0);
+    float2 sz = make_float2(0.f, 0.f);
+    if (in && row >= 0) {
+      piece = *reinterpret_cast<const uint4*>(codes + row * (a.G * 16) + j * 16);
+      sz.x = __half2float(scales[row * 2 * a.G + j]);
+      sz.y = __half2float(scales[row * 2 * a.G + a.G + j]);
+    }
+    *reinterpret_cast<uint4*>(words + lane * 8) = piece;
+    s_scale[warp][lane] = sz;
+    __syncwarp();
+    // eight values a lane: words 2 q and 2 q + 1 of a group; the step's rows lie on end in dst
+    const int total = min(rows, t1 - t0 - base) * a.G * 4;
+    for (int o = lane; o < total; o += 32) {
+      const int grp = o >> 2, rr = grp / a.G, jj = grp - rr * a.G, g = (o & 3) * 2;
+      const uint32_t w0 = words[rr * a.G * 8 + g * a.G + jj], w1 = words[rr * a.G * 8 + (g + 1) * a.G + jj];
+      const float2 c = s_scale[warp][grp];
+      // code e of both words at once: under the exponent of 1024 it is the fp16 1024 + n
+      T x[8];
+      const uint32_t w = w0 | w1 << 16;
 #pragma unroll
-    for (int i = 0; i < kInt4Flight; ++i) {
-      tt[i] = t;
-      jj[i] = j;
-      const int64_t row = __shfl_sync(0xffffffffu, my_row, t - t0 < 31 ? t - t0 : 31);
-      word[i] = 0;
-      s[i] = z[i] = 0.f;
-      if (t < t1 && row >= 0) {
-        word[i] = codes[row * (a.G * 8) + ln.g * a.G + j];
-        const __half* sc = scales + row * 2 * a.G + j;
-        s[i] = __half2float(sc[0]);
-        z[i] = __half2float(sc[a.G]);
+      for (int e = 0; e < 4; ++e) {
+        uint32_t y;
+        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(w >> (4 * e)), "r"(0x000f000fu), "r"(0x64006400u));
+        const float2 n = __half22float2(__hsub2(*reinterpret_cast<const __half2*>(&y), __float2half2_rn(1024.f)));
+        x[e] = from_f32<T>(fmaf(c.x, n.x, c.y));
+        x[4 + e] = from_f32<T>(fmaf(c.x, n.y, c.y));
       }
-      j += 4;
-      while (j >= a.G) j -= a.G, ++t;
+      T* p = dst + static_cast<int64_t>(t0 + base) * (a.G * kInt4Group) + o * 8;
+      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(x);
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(p + 4) = *reinterpret_cast<const uint4*>(x + 4);
     }
-#pragma unroll
-    for (int i = 0; i < kInt4Flight; ++i) {
-      if (tt[i] >= t1) continue;
-      T x[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = from_f32<T>(fmaf(s[i], static_cast<float>((word[i] >> (4 * e)) & 15u), z[i]));
-      T* p = dst + static_cast<int64_t>(tt[i]) * (a.G * kInt4Group) + jj[i] * kInt4Group + ln.g * 4;
-      if constexpr (sizeof(T) == 4)
-        *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(x);
-      else
-        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(x);
-    }
+    __syncwarp();
   }
 }
 
@@ -242,7 +259,7 @@ extern "C" int spa_int4_append(const spa_kv_layout* kv, void* k_scales, void* v_
   const spa::Int4Rows a = spa::int4_rows(*kv, k_scales, v_scales, batch, kv_heads, head_dim, tokens, positions, new_lens);
   const int64_t es = dtype_size(dtype);
   const int vec = (reinterpret_cast<uintptr_t>(k_new) | reinterpret_cast<uintptr_t>(v_new) | (stride_b * es) |
-                   (stride_h * es) | (stride_t * es)) % (4 * es) == 0;
+                   (stride_h * es) | (stride_t * es)) % 16 == 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const dim3 grid = spa::int4_grid(a);
   if (dtype == SPA_F32)
