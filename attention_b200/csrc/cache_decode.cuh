@@ -13,6 +13,7 @@
 
 #include "cache_args.cuh"
 #include "int4_mma.cuh"
+#include "plain_mma.cuh"
 
 namespace spa {
 
@@ -251,19 +252,20 @@ __global__ void __launch_bounds__(kFinishThreads) cache_decode_finish_kernel(con
 // ---------------------------------------------------------------------------
 // host planning
 constexpr int kWholeTiles = 24, kCtaTiles = 6;
+enum CacheKernel { kCachePlain, kCacheInt4Mma, kCachePlainMma };
 struct CachePlan {
-  bool mma;
-  int heads, chunks, ctas, slots;
+  int heads, chunks, ctas, slots, tile;
 };
-inline CachePlan cache_plan(int batch, int q_heads, int kv_heads, int head_dim, int max_candidates, bool mma) {
+inline CachePlan cache_plan(int batch, int q_heads, int kv_heads, int head_dim, int max_candidates, CacheKernel kind) {
   CachePlan p;
   const int group = q_heads / kv_heads;
-  p.mma = mma;
-  p.heads = mma ? int4_mma_heads(head_dim, group) : kPlainHeads;
+  p.heads = kind == kCachePlain ? kPlainHeads : kind == kCacheInt4Mma ? int4_mma_heads(head_dim, group) : 8;
   p.chunks = (group + p.heads - 1) / p.heads;
+  p.tile = kind == kCachePlainMma ? 16 : 32;
+  const int per_sm = kind == kCachePlain ? 4 : kind == kCacheInt4Mma ? int4_mma_ctas(head_dim, p.heads) : head_dim == 256 ? 1 : 2;
   const int64_t pairs = static_cast<int64_t>(batch) * kv_heads * p.chunks;
-  const int64_t tiles = (max_candidates + 31) / 32 + 1;
-  const int64_t room = static_cast<int64_t>(device_sm_count()) * (mma ? int4_mma_ctas(head_dim, p.heads) : 4);
+  const int64_t tiles = (max_candidates + p.tile - 1) / p.tile + 1;
+  const int64_t room = static_cast<int64_t>(device_sm_count()) * per_sm;
   const int64_t most = (pairs * tiles + kCtaTiles - 1) / kCtaTiles;
   // One CTA per pair where a pair has little to share, where pairs alone fill the GPU several
   // times over, or where the batch is longer than a CTA sums up.
@@ -316,8 +318,9 @@ int cache_decode_impl(CacheDecodeArgs a, int kv_dtype, const spa_kv_layout* kv, 
   a.group = a.Hq / a.Hkv;
   if (a.group > 256) return SPA_ERR_UNSUPPORTED;
   if (a.Hkv > 65535 || static_cast<int64_t>(a.B) * a.Hq > (1 << 28)) return SPA_ERR_UNSUPPORTED;
-  const CachePlan p =
-      cache_plan(a.B, a.Hq, a.Hkv, a.D, max_candidates, kv_dtype < 0 && int4_mma_serves(a.D, kv->total_rows));
+  const CacheKernel kind = kv_dtype < 0 ? (int4_mma_serves(a.D, kv->total_rows) ? kCacheInt4Mma : kCachePlain)
+                           : plain_mma_serves(kv_dtype, a.D, kv->k, kv->v, a.q) ? kCachePlainMma : kCachePlain;
+  const CachePlan p = cache_plan(a.B, a.Hq, a.Hkv, a.D, max_candidates, kind);
   const CacheScratch s = cache_scratch(p, a.B, a.Hq, a.D, a.cap, a.weights != nullptr);
   if (s.total && (!workspace || workspace_bytes < s.total || reinterpret_cast<uintptr_t>(workspace) % 16))
     return SPA_ERR_WORKSPACE;
@@ -337,8 +340,10 @@ int cache_decode_impl(CacheDecodeArgs a, int kv_dtype, const spa_kv_layout* kv, 
   a.scores = a.weights ? reinterpret_cast<float*>(ws + s.scores) : nullptr;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   int rc;
-  if (p.mma)
+  if (kind == kCacheInt4Mma)
     rc = launch_int4_decode(a, st);
+  else if (kind == kCachePlainMma)
+    rc = kv_dtype == SPA_F16 ? launch_plain_decode<__half>(a, st) : launch_plain_decode<__nv_bfloat16>(a, st);
   else if (kv_dtype < 0)
     rc = launch_cache_plain<uint8_t>(a, st);
   else if (kv_dtype == SPA_F32)
@@ -350,7 +355,8 @@ int cache_decode_impl(CacheDecodeArgs a, int kv_dtype, const spa_kv_layout* kv, 
   if (rc || !parts) return rc;
   const int span = a.local_window > 0 && a.local_window < a.cap ? a.local_window : a.cap;
   const int blocks = (a.group + kFinishHeads - 1) / kFinishHeads + (a.weights ? (span + kFinishTokens - 1) / kFinishTokens : 0);
-  SPA_CHECK_CUDA(launch_pdl(cache_decode_finish_kernel<32>, dim3(blocks, a.Hkv, a.B), dim3(kFinishThreads), 0, st, true, a));
+  SPA_CHECK_CUDA(launch_pdl(p.tile == 16 ? cache_decode_finish_kernel<16> : cache_decode_finish_kernel<32>,
+                            dim3(blocks, a.Hkv, a.B), dim3(kFinishThreads), 0, st, true, a));
   return SPA_OK;
 }
 
@@ -361,10 +367,11 @@ extern "C" size_t spa_cache_decode_workspace_size(int batch, int q_heads, int kv
   if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0 || max_candidates < 0 ||
       max_tokens <= 0)
     return 0;
-  // the number of rows decides between the kernels, and it is not known here: the larger need
+  // addresses and the number of rows decide between the kernels, and they are not known here:
+  // the larger need
   size_t most = 0;
-  for (int mma = 0; mma < (kv_dtype < 0 ? 2 : 1); ++mma) {
-    const spa::CachePlan p = spa::cache_plan(batch, q_heads, kv_heads, head_dim, max_candidates, mma != 0);
+  for (const spa::CacheKernel kind : {spa::kCachePlain, kv_dtype < 0 ? spa::kCacheInt4Mma : spa::kCachePlainMma}) {
+    const spa::CachePlan p = spa::cache_plan(batch, q_heads, kv_heads, head_dim, max_candidates, kind);
     const size_t need = spa::cache_scratch(p, batch, q_heads, head_dim, max_tokens, weights != 0).total;
     most = need > most ? need : most;
   }

@@ -15,57 +15,96 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// One CTA per (kv head, sequence).  The last r tokens stay; of the n = L - r before them the
-// `need` largest keys, ties to the lower token.  The need-th largest key is found digit by
-// digit (11, 11 and 10 bits, a histogram each), then one pass in token order writes the
-// tokens above it and the first of those equal to it.
-constexpr int kSelThreads = 1024;
+// A cluster of CTAs per (kv head, sequence), each with a stretch of its tokens.  The last r
+// tokens stay; of the n = L - r before them the `need` largest keys, ties to the lower token.
+// The need-th largest key is found digit by digit (11, 11 and 10 bits): every CTA counts its
+// keys' digits in shared memory and all add up the cluster's counts.  Then one pass in token
+// order writes the tokens above that key and the first of those equal to it, each CTA from the
+// number that the CTAs before it hold.
+//
+// Weights are read once and stay in shared memory as keys (longer stretches than that holds are
+// read again).  What bounds it: the latency of those four rounds; one CTA a pair took 72 us for
+// 64 rows of 32768.
+constexpr int kSelThreads = 512, kSelBins = 2048, kSelSlice = 4 * kSelThreads;
+constexpr int kSelCached = 40 * 1024;  // keys a CTA keeps
 
+__device__ __forceinline__ int ld_dsmem(const int* local, int rank) {
+  uint32_t ra;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(smem_u32(local)), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(ra) : "memory");
+  return v;
+}
+
+template <bool CACHED>
 __global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(const float* __restrict__ weights, int T,
                                                                     const int32_t* __restrict__ lens, int budget,
                                                                     int recent, int32_t* __restrict__ keep,
                                                                     int32_t* __restrict__ kept_lens) {
-  __shared__ int hist[2048];
-  __shared__ int wsum[kSelThreads / 32][2];
+  extern __shared__ uint32_t s_key[];
+  __shared__ int hist[kSelBins], count[2];
+  __shared__ int warp_sum[kSelThreads / 32];
   __shared__ uint32_t s_prefix;
   __shared__ int s_need;
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t bh = static_cast<int64_t>(b) * gridDim.x + h;
+  uint32_t rank, ranks;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
+  asm volatile("mov.u32 %0, %cluster_nctarank;" : "=r"(ranks));
+  const int h = blockIdx.x / ranks, heads = gridDim.x / ranks, b = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, all = ranks * kSelThreads, me = rank * kSelThreads + tid;
+  const int64_t bh = static_cast<int64_t>(b) * heads + h;
   const float* w = weights + bh * T;
   int32_t* out = keep + bh * budget;
   const int L = min(max(lens[b], 0), T);
-  if (h == 0 && tid == 0) kept_lens[b] = min(L, budget);
-  if (L <= budget) {
-    for (int i = tid; i < budget; i += kSelThreads) out[i] = i < L ? i : -1;
+  if (h == 0 && me == 0) kept_lens[b] = min(L, budget);
+  if (L <= budget) {  // the same for the whole cluster
+    for (int i = me; i < budget; i += all) out[i] = i < L ? i : -1;
     return;
   }
   const int r = min(recent, budget), n = L - r, need0 = budget - r;
-  for (int i = tid; i < r; i += kSelThreads) out[need0 + i] = n + i;
+  for (int i = me; i < r; i += all) out[need0 + i] = n + i;
   if (need0 == 0) return;
+  const int span = (n + ranks - 1) / ranks, lo = min(static_cast<int>(rank) * span, n), m = min(span, n - lo);
+  const auto key = [&](int i) { return CACHED ? s_key[i] : weight_key(w[lo + i]); };
+  for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
+  if constexpr (CACHED) {
+#pragma unroll 4
+    for (int i = tid; i < m; i += kSelThreads) s_key[i] = weight_key(w[lo + i]);
+  }
+  __syncthreads();
   uint32_t prefix = 0, mask = 0;
   int need = need0;
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-    for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += kSelThreads) {
-      const uint32_t k = weight_key(w[i]);
+#pragma unroll 4
+    for (int i = tid; i < m; i += kSelThreads) {
+      const uint32_t k = key(i);
       if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1);
     }
     __syncthreads();
+    cluster_barrier();
+    int sum[kSelBins / kSelThreads];
+#pragma unroll
+    for (int u = 0; u < kSelBins / kSelThreads; ++u) {
+      sum[u] = hist[u * kSelThreads + tid];
+      for (uint32_t o = 1; o < ranks; ++o) sum[u] += ld_dsmem(hist + u * kSelThreads + tid, (rank + o) % ranks);
+    }
+    cluster_barrier();  // all have read: the counts may become the cluster's
+#pragma unroll
+    for (int u = 0; u < kSelBins / kSelThreads; ++u) hist[u * kSelThreads + tid] = sum[u];
+    __syncthreads();
     if (warp == 0) {
-      // from the top bin down, 64 bins per lane, until `need` keys are covered
+      // from the top bin down, 1/32 of the bins a lane, until `need` keys are covered
       const int per = (1 << bits) / 32, top = (1 << bits) - 1 - lane * per;
-      int sum = 0;
-      for (int i = 0; i < per; ++i) sum += hist[top - i];
-      int inc = sum;
+      int total = 0;
+      for (int i = 0; i < per; ++i) total += hist[top - i];
+      int inc = total;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
         const int o = __shfl_up_sync(0xffffffffu, inc, off);
         if (lane >= off) inc += o;
       }
-      int before = inc - sum;
+      int before = inc - total;
       if (before < need && inc >= need) {
         int i = 0;
         while (before + hist[top - i] < need) before += hist[top - i++];
@@ -77,33 +116,67 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(const float*
     prefix = s_prefix;
     need = s_need;
     mask |= ((1u << bits) - 1) << shift;
+    for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
+    __syncthreads();
   }
-  // tokens above the threshold and the first `need` equal to it, in token order
+  // tokens above the key and equal to it here and in the CTAs before
+  int mine[2] = {0, 0};
+#pragma unroll 4
+  for (int i = tid; i < m; i += kSelThreads) {
+    const uint32_t k = key(i);
+    mine[0] += k > prefix;
+    mine[1] += k == prefix;
+  }
+  if (tid < 2) count[tid] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int x = __reduce_add_sync(0xffffffffu, mine[u]);
+    if (lane == 0) atomicAdd(&count[u], x);
+  }
+  __syncthreads();
+  cluster_barrier();
   int above0 = 0, equal0 = 0;
-  for (int base = 0; base < n; base += kSelThreads) {
-    const int i = base + tid;
-    const uint32_t k = i < n ? weight_key(w[i]) : 0u;
-    const bool gt = i < n && k > prefix, eq = i < n && k == prefix;
-    const unsigned bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) {
-      wsum[warp][0] = __popc(bg);
-      wsum[warp][1] = __popc(be);
+  for (uint32_t o = 0; o < rank; ++o) above0 += ld_dsmem(count, o), equal0 += ld_dsmem(count + 1, o);
+  // token order: four tokens a thread; both counts of a slice fit 16 bits
+  for (int base = 0; base < m; base += kSelSlice) {
+    const int i0 = base + 4 * tid;
+    uint32_t k[4];
+    int c = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      k[e] = i0 + e < m ? key(i0 + e) : 0u;
+      const bool in = i0 + e < m;
+      c += (in && k[e] > prefix ? 1 : 0) + (in && k[e] == prefix ? 1 << 16 : 0);
     }
+    int inc = c;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, inc, off);
+      if (lane >= off) inc += o;
+    }
+    if (lane == 31) warp_sum[warp] = inc;
     __syncthreads();
-    int above = above0, equal = equal0, ta = 0, te = 0;
+    int before = inc - c, total = 0;
+#pragma unroll
     for (int v = 0; v < kSelThreads / 32; ++v) {
-      if (v < warp) above += wsum[v][0], equal += wsum[v][1];
-      ta += wsum[v][0];
-      te += wsum[v][1];
+      if (v < warp) before += warp_sum[v];
+      total += warp_sum[v];
     }
-    const unsigned lt = (1u << lane) - 1;
-    above += __popc(bg & lt);
-    equal += __popc(be & lt);
-    if (gt || (eq && equal < need)) out[above + min(equal, need)] = i;
-    above0 += ta;
-    equal0 += te;
+    int above = above0 + (before & 0xffff), equal = equal0 + (before >> 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (i0 + e >= m) continue;
+      const bool gt = k[e] > prefix, eq = k[e] == prefix;
+      if (gt || (eq && equal < need)) out[above + min(equal, need)] = lo + i0 + e;
+      above += gt;
+      equal += eq;
+    }
+    above0 += total & 0xffff;
+    equal0 += total >> 16;
     __syncthreads();
   }
+  cluster_barrier();  // no CTA leaves while its counts may still be read
 }
 
 // In-place compaction.  Of one (sequence, kv head) row j <- row keep[j] with keep ascending,
@@ -294,12 +367,20 @@ __global__ void __launch_bounds__(kCompactThreads, 4) compact_kernel(const Compa
 
 extern "C" int spa_select_tokens(const float* weights, int batch, int kv_heads, int tokens, const int32_t* lens,
                                  int budget, int recent, int32_t* keep, int32_t* kept_lens, spa_stream_t stream) {
-  if (!weights || !lens || !keep || !kept_lens || batch <= 0 || batch > 65535 || kv_heads <= 0 || tokens <= 0 ||
+  if (!weights || !lens || !keep || !kept_lens || batch <= 0 || batch > 65535 || kv_heads <= 0 || kv_heads > (1 << 20) || tokens <= 0 ||
       budget <= 0 || recent < 0)
     return SPA_ERR_INVALID;
-  spa::select_tokens_kernel<<<dim3(kv_heads, batch), spa::kSelThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-      weights, tokens, lens, budget, recent, keep, kept_lens);
-  SPA_CHECK_CUDA(cudaGetLastError());
+  // CTAs a cluster: a slice each at least, up to the portable 8
+  const int slices = (tokens + spa::kSelSlice - 1) / spa::kSelSlice;
+  const int ranks = slices >= 8 ? 8 : slices >= 4 ? 4 : slices >= 2 ? 2 : 1;
+  const int span = (tokens + ranks - 1) / ranks;
+  const bool cached = span <= spa::kSelCached;
+  const size_t smem = cached ? sizeof(uint32_t) * static_cast<size_t>(span) : 0;
+  auto kern = cached ? spa::select_tokens_kernel<true> : spa::select_tokens_kernel<false>;
+  SPA_CHECK_CUDA(spa_set_smem_once(kern, static_cast<int>(smem)));
+  SPA_CHECK_CUDA(spa::launch_ex(kern, dim3(kv_heads * ranks, batch), dim3(spa::kSelThreads), smem,
+                                reinterpret_cast<cudaStream_t>(stream), false, ranks, weights, tokens, lens, budget,
+                                recent, keep, kept_lens));
   return SPA_OK;
 }
 

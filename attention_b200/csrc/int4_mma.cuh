@@ -648,40 +648,7 @@ __global__ void __launch_bounds__(Int4Cfg<G, NT>::kWarps * 32, Int4Cfg<G, NT>::k
       }
     }
   }
-  __syncthreads();
-  const bool partial = a.weights || !seg.whole;
-  if (tid < HN * 16) {  // a head's warps side by side: their shares of the whole
-    const int n = tid >> 4, w = tid & 15;
-    const float* row = buf + (w * HN + n) * kLd + D;
-    const float mw = w < W ? row[0] : -INFINITY, lw = w < W ? row[1] : 0.f;
-    float M = mw;
-#pragma unroll
-    for (int off = 1; off < 16; off <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-    const float f = mw == -INFINITY ? 0.f : fast_exp2(mw - M);
-    float sum = lw * f;
-#pragma unroll
-    for (int off = 1; off < 16; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    // no token at all (sum 0): zeros
-    s_f[n][w] = sum == 0.f ? 0.f : f / sum;
-    if (partial && w == 0 && n < heads)
-      a.part_lse[static_cast<int64_t>(seg.slot) * HN + n] = sum == 0.f ? -INFINITY : M + log2f(sum);
-  }
-  __syncthreads();
-#pragma unroll 1
-  for (int i = tid; i < heads * (D / 4); i += W * 32) {
-    const int n = i / (D / 4), d = i % (D / 4) * 4;
-    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int w = 0; w < W; ++w) {
-      const float f = s_f[n][w];
-      const float4 v = *reinterpret_cast<const float4*>(buf + (w * HN + n) * kLd + d);
-      r.x = fmaf(v.x, f, r.x), r.y = fmaf(v.y, f, r.y), r.z = fmaf(v.z, f, r.z), r.w = fmaf(v.w, f, r.w);
-    }
-    if (partial)
-      *reinterpret_cast<float4*>(a.part_o + (static_cast<int64_t>(seg.slot) * HN + n) * D + d) = r;
-    else
-      store4_any(a.out, a.dtype, (q0 + n) * D + d, r);
-  }
+  merge_warps<W, HN, D>(a, seg, q0, heads, buf, s_f);
   __syncthreads();  // the next segment's loads reuse the buffer
   }
 }
