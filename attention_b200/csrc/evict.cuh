@@ -17,15 +17,16 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 
 // A cluster of CTAs per (kv head, sequence), each with a stretch of its tokens.  The last r
 // tokens stay; of the n = L - r before them the `need` largest keys, ties to the lower token.
-// The need-th largest key is found digit by digit (11, 11 and 10 bits): every CTA counts its
-// keys' digits in shared memory and all add up the cluster's counts.  Then one pass in token
-// order writes the tokens above that key and the first of those equal to it, each CTA from the
-// number that the CTAs before it hold.
+// The need-th largest key is found byte by byte: every CTA counts its keys' bytes in shared
+// memory and all add up the cluster's counts (256 bins: the exchange is 7 KB a CTA and byte; with
+// 11 bits at a time it was 57 KB and took as long as the counting).  The first byte is mostly
+// exponent, a few values for all keys, so a warp's lanes count it in eight copies.  Then one pass in token order writes the tokens above that key and the first of those equal to it, each
+// CTA from the number that the CTAs before it hold.
 //
 // Weights are read once and stay in shared memory as keys (longer stretches than that holds are
 // read again).  What bounds it: the latency of those four rounds; one CTA a pair took 72 us for
 // 64 rows of 32768.
-constexpr int kSelThreads = 512, kSelBins = 2048, kSelSlice = 4 * kSelThreads;
+constexpr int kSelThreads = 512, kSelBins = 256, kSelSlice = 4 * kSelThreads;
 constexpr int kSelCached = 40 * 1024;  // keys a CTA keeps
 
 __device__ __forceinline__ int ld_dsmem(const int* local, int rank) {
@@ -37,12 +38,14 @@ __device__ __forceinline__ int ld_dsmem(const int* local, int rank) {
 }
 
 template <bool CACHED>
-__global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(const float* __restrict__ weights, int T,
+__global__ void __launch_bounds__(kSelThreads, 4) select_tokens_kernel(const float* __restrict__ weights, int T,
                                                                     const int32_t* __restrict__ lens, int budget,
                                                                     int recent, int32_t* __restrict__ keep,
                                                                     int32_t* __restrict__ kept_lens) {
   extern __shared__ uint32_t s_key[];
-  __shared__ int hist[kSelBins], count[2];
+  __shared__ int hist[4][kSelBins];  // of each byte
+  __shared__ __align__(16) int copies[2][kSelBins][8];
+  __shared__ int count[2];
   __shared__ int warp_sum[kSelThreads / 32];
   __shared__ uint32_t s_prefix;
   __shared__ int s_need;
@@ -65,7 +68,8 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(const float*
   if (need0 == 0) return;
   const int span = (n + ranks - 1) / ranks, lo = min(static_cast<int>(rank) * span, n), m = min(span, n - lo);
   const auto key = [&](int i) { return CACHED ? s_key[i] : weight_key(w[lo + i]); };
-  for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
+  for (int i = tid; i < 4 * kSelBins; i += kSelThreads) hist[0][i] = 0;
+  for (int i = tid; i < 4 * kSelBins; i += kSelThreads) reinterpret_cast<int4*>(copies)[i] = make_int4(0, 0, 0, 0);
   if constexpr (CACHED) {
 #pragma unroll 4
     for (int i = tid; i < m; i += kSelThreads) s_key[i] = weight_key(w[lo + i]);
@@ -74,50 +78,57 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(const float*
   uint32_t prefix = 0, mask = 0;
   int need = need0;
 #pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+  for (int pass = 0; pass < 4; ++pass) {
+    const int shift = 24 - 8 * pass;
+    if (pass < 2) {
 #pragma unroll 4
-    for (int i = tid; i < m; i += kSelThreads) {
-      const uint32_t k = key(i);
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1);
+      for (int i = tid; i < m; i += kSelThreads) {
+        const uint32_t k = key(i);
+        if ((k & mask) == prefix) atomicAdd(&copies[pass][(k >> shift) & 0xffu][lane & 7], 1);
+      }
+      __syncthreads();
+      if (tid < kSelBins) {
+        const int4 c = reinterpret_cast<const int4*>(copies[pass][tid])[0], d = reinterpret_cast<const int4*>(copies[pass][tid])[1];
+        hist[pass][tid] = c.x + c.y + c.z + c.w + d.x + d.y + d.z + d.w;
+      }
+    } else {
+#pragma unroll 4
+      for (int i = tid; i < m; i += kSelThreads) {
+        const uint32_t k = key(i);
+        if ((k & mask) == prefix) atomicAdd(&hist[pass][(k >> shift) & 0xffu], 1);
+      }
     }
-    __syncthreads();
     cluster_barrier();
-    int sum[kSelBins / kSelThreads];
+    // a bin a thread, over the cluster
+    int total = 0, x[8];
+    if (tid < kSelBins) {
 #pragma unroll
-    for (int u = 0; u < kSelBins / kSelThreads; ++u) {
-      sum[u] = hist[u * kSelThreads + tid];
-      for (uint32_t o = 1; o < ranks; ++o) sum[u] += ld_dsmem(hist + u * kSelThreads + tid, (rank + o) % ranks);
+      for (int o = 0; o < 8; ++o)
+        x[o] = o < static_cast<int>(ranks) ? ld_dsmem(&hist[pass][tid], (rank + o) & (ranks - 1)) : 0;
+#pragma unroll
+      for (int o = 0; o < 8; ++o) total += x[o];
     }
-    cluster_barrier();  // all have read: the counts may become the cluster's
+    // keys in higher bins: of higher lanes, and of higher warps
+    int above = total;
 #pragma unroll
-    for (int u = 0; u < kSelBins / kSelThreads; ++u) hist[u * kSelThreads + tid] = sum[u];
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_down_sync(0xffffffffu, above, off);
+      if (lane + off < 32) above += o;
+    }
+    if (lane == 0) warp_sum[warp] = above;
+    above -= total;
     __syncthreads();
-    if (warp == 0) {
-      // from the top bin down, 1/32 of the bins a lane, until `need` keys are covered
-      const int per = (1 << bits) / 32, top = (1 << bits) - 1 - lane * per;
-      int total = 0;
-      for (int i = 0; i < per; ++i) total += hist[top - i];
-      int inc = total;
 #pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, inc, off);
-        if (lane >= off) inc += o;
-      }
-      int before = inc - total;
-      if (before < need && inc >= need) {
-        int i = 0;
-        while (before + hist[top - i] < need) before += hist[top - i++];
-        s_prefix = prefix | (static_cast<uint32_t>(top - i) << shift);
-        s_need = need - before;
-      }
+    for (int v = 1; v < kSelBins / 32; ++v)
+      if (v > warp) above += warp_sum[v];
+    if (tid < kSelBins && above < need && above + total >= need) {  // one thread
+      s_prefix = prefix | static_cast<uint32_t>(tid) << shift;
+      s_need = need - above;
     }
     __syncthreads();
     prefix = s_prefix;
     need = s_need;
-    mask |= ((1u << bits) - 1) << shift;
-    for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
-    __syncthreads();
+    mask |= 0xffu << shift;
   }
   // tokens above the key and equal to it here and in the CTAs before
   int mine[2] = {0, 0};
@@ -136,8 +147,9 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(const float*
   }
   __syncthreads();
   cluster_barrier();
-  int above0 = 0, equal0 = 0;
-  for (uint32_t o = 0; o < rank; ++o) above0 += ld_dsmem(count, o), equal0 += ld_dsmem(count + 1, o);
+  const bool before_me = lane < static_cast<int>(rank);
+  int above0 = __reduce_add_sync(0xffffffffu, before_me ? ld_dsmem(count, lane) : 0);
+  int equal0 = __reduce_add_sync(0xffffffffu, before_me ? ld_dsmem(count + 1, lane) : 0);
   // token order: four tokens a thread; both counts of a slice fit 16 bits
   for (int base = 0; base < m; base += kSelSlice) {
     const int i0 = base + 4 * tid;
