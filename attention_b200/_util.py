@@ -3,8 +3,6 @@ per-device cached buffers (workspaces, constant length vectors)."""
 
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
 from . import _lib
@@ -27,12 +25,13 @@ def stream_ptr(device: torch.device | int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-_SAME_DEVICE = contextlib.nullcontext()
-
-
-def on_device(device: torch.device):
-    """Makes ``device`` the current one for a launch (free when it already is)."""
-    return _SAME_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def launch(fn, device: int, *args) -> int:
+    """Calls the C entry point ``fn(*args, stream)`` with CUDA device ``device`` current, on the
+    caller's stream of that device."""
+    if device == torch._C._cuda_getDevice():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    with torch.cuda.device(device):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(device))
 
 
 def require_cuda(*tensors: torch.Tensor, message: str = "CUDA tensors are required") -> None:

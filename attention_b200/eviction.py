@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._util import as_int32, on_device, stream_ptr
+from ._util import as_int32, launch
 
 
 def select_tokens(weights: torch.Tensor, context_lens: torch.Tensor, *, budget: int,
@@ -32,15 +32,14 @@ def select_tokens(weights: torch.Tensor, context_lens: torch.Tensor, *, budget: 
     if budget <= 0 or recent < 0:
         raise ValueError("budget must be positive and recent >= 0")
     batch, heads, tokens = weights.shape
-    dev = weights.device
+    dev = weights.get_device()
     lens = as_int32(context_lens).contiguous()
-    if lens.shape != (batch,) or lens.device != dev:
+    if lens.dim() != 1 or lens.size(0) != batch or lens.get_device() != dev:
         raise ValueError("context_lens must be [batch] on the weights' device")
-    keep = torch.empty(batch, heads, budget, dtype=torch.int32, device=dev)
-    kept = torch.empty(batch, dtype=torch.int32, device=dev)
-    with on_device(dev):
-        rc = _lib.lib.spa_select_tokens(weights.data_ptr(), batch, heads, tokens, lens.data_ptr(), budget, recent,
-                                        keep.data_ptr(), kept.data_ptr(), stream_ptr(dev))
+    keep = torch.empty((batch, heads, budget), dtype=torch.int32, device=weights.device)
+    kept = torch.empty_like(lens)
+    rc = launch(_lib.lib.spa_select_tokens, dev, weights.data_ptr(), batch, heads, tokens, lens.data_ptr(), budget,
+                recent, keep.data_ptr(), kept.data_ptr())
     _lib.check(rc, "spa_select_tokens")
     return keep, kept
 
@@ -58,35 +57,37 @@ def compact_tokens(pools, page_table: torch.Tensor, keep: torch.Tensor, *,
     flat = [t for p in pools for t in (p if isinstance(p, (tuple, list)) else (p,))]
     if not flat or len(flat) > 8:
         raise ValueError("pools must hold 1 to 8 tensors")
-    if not all(t.is_cuda for t in (*flat, page_table, keep)):
+    dev = keep.get_device()
+    shape = flat[0].shape
+    ptrs, sizes = (ctypes.c_void_p * len(flat))(), (ctypes.c_int * len(flat))()
+    if dev < 0 or page_table.get_device() < 0:
         raise ValueError("CUDA tensors are required")
-    dev = keep.device
-    if any(t.device != dev for t in (*flat, page_table)):
+    for i, t in enumerate(flat):
+        if t.get_device() != dev:
+            raise ValueError("CUDA tensors are required" if not t.is_cuda else "tensors must be on one device")
+        if t.dim() < 4 or t.shape[:3] != shape[:3] or t.numel() == 0:
+            raise ValueError("pools must be [pages, Hkv, P, ...] of one geometry")
+        if not t.is_contiguous():
+            raise ValueError("contiguous CUDA tensors are required")
+        ptrs[i], sizes[i] = t.data_ptr(), t.stride(2) * t.element_size()
+    if page_table.get_device() != dev:
         raise ValueError("tensors must be on one device")
-    if any(t.dim() < 4 or t.shape[:3] != flat[0].shape[:3] or t.numel() == 0 for t in flat):
-        raise ValueError("pools must be [pages, Hkv, P, ...] of one geometry")
-    if not all(t.is_contiguous() for t in flat):
-        raise ValueError("contiguous CUDA tensors are required")
     if keep.dtype != torch.int32 or keep.dim() != 3 or keep.numel() == 0 or not keep.is_contiguous():
         raise ValueError("keep must be a contiguous int32 tensor [batch, kv_heads, budget]")
     table = as_int32(page_table).contiguous()
-    pages, heads, page = flat[0].shape[:3]
-    batch = keep.size(0)
-    if keep.size(1) != heads or table.dim() != 2 or table.size(0) != batch or table.size(1) == 0:
+    pages, heads, page = shape[:3]
+    batch, kept_heads, budget = keep.shape
+    if kept_heads != heads or table.dim() != 2 or table.size(0) != batch or table.size(1) == 0:
         raise ValueError("keep must be [batch, kv_heads, budget] and page_table [batch, pages]")
     if weights is not None and (weights.dtype != torch.float32 or weights.dim() != 3
-                                or weights.shape[:2] != keep.shape[:2] or weights.size(2) < keep.size(2)
-                                or not weights.is_contiguous() or weights.device != dev):
+                                or weights.shape[:2] != (batch, heads) or weights.size(2) < budget
+                                or not weights.is_contiguous() or weights.get_device() != dev):
         raise ValueError("weights must be a contiguous float32 tensor [batch, kv_heads, tokens >= budget]")
-    n = len(flat)
     layout = _lib.KvLayout(None, None, pages * heads * page, 0, heads * page, page, table.data_ptr(), table.size(1),
                            page)
-    ptrs = (ctypes.c_void_p * n)(*(t.data_ptr() for t in flat))
-    sizes = (ctypes.c_int * n)(*(t.stride(2) * t.element_size() for t in flat))
-    with on_device(dev):
-        rc = _lib.lib.spa_compact_tokens(ctypes.byref(layout), n, ptrs, sizes, batch, heads, keep.data_ptr(),
-                                         keep.size(2), weights.data_ptr() if weights is not None else None,
-                                         weights.size(2) if weights is not None else 0, stream_ptr(dev))
+    rc = launch(_lib.lib.spa_compact_tokens, dev, ctypes.byref(layout), len(flat), ptrs, sizes, batch, heads,
+                keep.data_ptr(), budget, weights.data_ptr() if weights is not None else None,
+                weights.size(2) if weights is not None else 0)
     _lib.check(rc, "spa_compact_tokens")
 
 

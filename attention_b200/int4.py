@@ -19,7 +19,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._util import as_int32, as_int64, dtype_code, on_device, stream_ptr
+from ._util import as_int32, as_int64, dtype_code, launch
 
 GROUP = 32
 
@@ -52,37 +52,46 @@ def int4_values(pool: tuple[torch.Tensor, torch.Tensor]) -> torch.Tensor:
     return (n * scale[..., None] + zero[..., None]).flatten(-2).float()
 
 
+def _same_device(device: int, *tensors) -> None:
+    for t in tensors:
+        if t.get_device() != device:
+            raise ValueError("CUDA tensors are required" if not t.is_cuda else "tensors must be on one device")
+
+
 def _pools(k_pool, v_pool, page_table):
-    """Checks two 4-bit pools and returns (layout, kv_heads, head_dim, page table kept alive)."""
+    """Checks two 4-bit pools and returns (layout, the scales' addresses, kv_heads, head_dim, page
+    table kept alive, device index)."""
     for pool in (k_pool, v_pool):
         if not isinstance(pool, (tuple, list)) or len(pool) != 2:
             raise ValueError("a 4-bit pool is a pair (codes, scales)")
     (kc, ks), (vc, vs) = k_pool, v_pool
-    if not (kc.is_cuda and ks.is_cuda and vc.is_cuda and vs.is_cuda and page_table.is_cuda):
+    dev = kc.get_device()
+    if dev < 0:
         raise ValueError("CUDA tensors are required")
+    _same_device(dev, ks, vc, vs, page_table)
     if kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or ks.dtype != torch.float16 or vs.dtype != torch.float16:
         raise ValueError("a 4-bit pool holds uint8 codes and float16 scales")
-    n, h, p, half = kc.shape if kc.dim() == 4 else (0, 0, 0, 0)
-    if half == 0 or half % 16 or half > 128 or vc.shape != kc.shape:
+    shape = kc.shape
+    n, h, p, half = shape if len(shape) == 4 else (0, 0, 0, 0)
+    if half == 0 or half % 16 or half > 128 or vc.shape != shape:
         raise ValueError("codes must be [pages, Hkv, P, D/2] with D a multiple of 32 up to 256")
     if ks.shape != (n, h, p, 2, half // 16) or vs.shape != ks.shape:
         raise ValueError("scales must be [pages, Hkv, P, 2, D/32]")
     if not (kc.is_contiguous() and ks.is_contiguous() and vc.is_contiguous() and vs.is_contiguous()):
         raise ValueError("contiguous CUDA tensors are required")
-    if len({t.device for t in (kc, ks, vc, vs, page_table)}) != 1:
-        raise ValueError("tensors must be on one device")
-    if (kc.data_ptr() | ks.data_ptr() | vc.data_ptr() | vs.data_ptr()) % 16:
+    kp, vp, ksp, vsp = kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr()
+    if (kp | vp | ksp | vsp) % 16:
         raise ValueError("4-bit pools must be 16-byte aligned")
     table = as_int32(page_table).contiguous()
     if table.dim() != 2 or table.size(1) == 0:
         raise ValueError("page_table must be [batch, pages]")
-    layout = _lib.KvLayout(kc.data_ptr(), vc.data_ptr(), n * h * p, 0, h * p, p, table.data_ptr(), table.size(1), p)
-    return layout, h, 2 * half, table
+    layout = _lib.KvLayout(kp, vp, n * h * p, 0, h * p, p, table.data_ptr(), table.size(1), p)
+    return layout, ksp, vsp, h, 2 * half, table, dev
 
 
-def _lengths(t, batch: int, dev, name: str) -> torch.Tensor:
+def _lengths(t, batch: int, dev: int, name: str) -> torch.Tensor:
     out = as_int32(t).contiguous()
-    if out.shape != (batch,) or out.device != dev:
+    if out.dim() != 1 or out.size(0) != batch or out.get_device() != dev:
         raise ValueError(f"{name} must be [batch] on the pools' device")
     return out
 
@@ -92,28 +101,26 @@ def kv_append_int4(k_pool, v_pool, page_table: torch.Tensor, k_new: torch.Tensor
     """Quantises ``k_new``/``v_new`` ``[B, Hkv, D]`` (one token) or ``[B, Hkv, T, D]`` into the
     tokens from ``positions[b]`` on; with ``new_lens`` only the first ``new_lens[b]`` of the T.
     The new tensors may be views with any strides over B, Hkv and T (both the same)."""
-    layout, kv_heads, dim, table = _pools(k_pool, v_pool, page_table)
-    dev, batch = table.device, table.size(0)
-    if not (k_new.is_cuda and v_new.is_cuda and positions.is_cuda):
-        raise ValueError("CUDA tensors are required")
-    if k_new.dim() == 3 and v_new.dim() == 3:
-        k_new, v_new = k_new.unsqueeze(2), v_new.unsqueeze(2)
-    if k_new.dim() != 4 or v_new.shape != k_new.shape or k_new.size(1) != kv_heads or k_new.size(3) != dim:
+    layout, k_scales, v_scales, kv_heads, dim, table, dev = _pools(k_pool, v_pool, page_table)
+    batch = table.size(0)
+    _same_device(dev, k_new, v_new, positions)
+    shape, strides = k_new.shape, k_new.stride()
+    tokens = 1
+    if len(shape) == 4:
+        tokens = shape[2]
+    if (len(shape) not in (3, 4) or v_new.shape != shape or shape[1] != kv_heads or shape[-1] != dim):
         raise ValueError("k_new/v_new must be [B, Hkv, D] or [B, Hkv, T, D]")
-    if k_new.size(0) != batch or v_new.dtype != k_new.dtype:
+    if shape[0] != batch or v_new.dtype != k_new.dtype:
         raise ValueError("k_new/v_new must match the page table's batch and each other's dtype")
-    if k_new.device != dev or v_new.device != dev:
-        raise ValueError("tensors must be on one device")
     code = dtype_code(k_new)
-    if k_new.stride(3) != 1 or k_new.stride() != v_new.stride():
+    if strides[-1] != 1 or strides != v_new.stride():
         k_new, v_new = k_new.contiguous(), v_new.contiguous()
+        strides = k_new.stride()
     pos = _lengths(positions, batch, dev, "positions")
     lens = _lengths(new_lens, batch, dev, "new_lens") if new_lens is not None else None
-    sb, sh, st, _ = k_new.stride()
-    with on_device(dev):
-        rc = _lib.lib.spa_int4_append(ctypes.byref(layout), k_pool[1].data_ptr(), v_pool[1].data_ptr(), code, batch,
-                                      kv_heads, dim, k_new.size(2), k_new.data_ptr(), v_new.data_ptr(), sb, sh, st,
-                                      pos.data_ptr(), lens.data_ptr() if lens is not None else None, stream_ptr(dev))
+    rc = launch(_lib.lib.spa_int4_append, dev, ctypes.byref(layout), k_scales, v_scales, code, batch, kv_heads, dim,
+                tokens, k_new.data_ptr(), v_new.data_ptr(), strides[0], strides[1],
+                strides[2] if len(shape) == 4 else 0, pos.data_ptr(), lens.data_ptr() if lens is not None else None)
     _lib.check(rc, "spa_int4_append")
 
 
@@ -123,38 +130,32 @@ def kv_read_int4(k_pool, v_pool, page_table: torch.Tensor, positions: torch.Tens
     """The values of tokens ``positions[b] + [0, tokens)`` as contiguous K and V
     ``[B, Hkv, tokens, D]`` of ``dtype`` (a cached prefix for ``local_causal_prefill``); zeros
     past ``lens[b]`` and for tokens without a page."""
-    layout, kv_heads, dim, table = _pools(k_pool, v_pool, page_table)
-    dev, batch = table.device, table.size(0)
+    layout, k_scales, v_scales, kv_heads, dim, table, dev = _pools(k_pool, v_pool, page_table)
+    batch = table.size(0)
     if tokens < 0:
         raise ValueError("tokens must be >= 0")
     pos = _lengths(positions, batch, dev, "positions")
     n = _lengths(lens, batch, dev, "lens") if lens is not None else None
-    k = torch.empty(batch, kv_heads, tokens, dim, dtype=dtype, device=dev)
+    k = torch.empty((batch, kv_heads, tokens, dim), dtype=dtype, device=table.device)
     v = torch.empty_like(k)
-    with on_device(dev):
-        rc = _lib.lib.spa_int4_read(ctypes.byref(layout), k_pool[1].data_ptr(), v_pool[1].data_ptr(), dtype_code(k),
-                                    batch, kv_heads, dim, tokens, pos.data_ptr(),
-                                    n.data_ptr() if n is not None else None, k.data_ptr(), v.data_ptr(),
-                                    stream_ptr(dev))
+    rc = launch(_lib.lib.spa_int4_read, dev, ctypes.byref(layout), k_scales, v_scales, dtype_code(k), batch, kv_heads,
+                dim, tokens, pos.data_ptr(), n.data_ptr() if n is not None else None, k.data_ptr(), v.data_ptr())
     _lib.check(rc, "spa_int4_read")
     return k, v
 
 
-def check_weights(weights, batch: int, kv_heads: int, dev) -> None:
+def check_weights(weights, batch: int, kv_heads: int, dev: int) -> None:
     """``weights`` must be fp32 ``[B, Hkv, T]``, written in place."""
     if (not isinstance(weights, torch.Tensor) or weights.dtype != torch.float32 or weights.dim() != 3
             or weights.shape[:2] != (batch, kv_heads) or weights.size(2) == 0 or not weights.is_contiguous()
-            or weights.device != dev):
+            or weights.get_device() != dev):
         raise ValueError("weights must be a contiguous float32 tensor [batch, kv_heads, tokens] on the query's device")
 
 
 def _decode(query, k_pool, v_pool, page_table, context_lens, local_window, selected, weights, block_size=None):
-    layout, kv_heads, dim, table = _pools(k_pool, v_pool, page_table)
-    dev, page = table.device, layout.page_size
-    if not query.is_cuda:
-        raise ValueError("CUDA tensors are required")
-    if query.device != dev:
-        raise ValueError("tensors must be on one device")
+    layout, k_scales, v_scales, kv_heads, dim, table, dev = _pools(k_pool, v_pool, page_table)
+    page = layout.page_size
+    _same_device(dev, query)
     if not query.is_contiguous():
         raise ValueError("contiguous CUDA tensors are required")
     if query.dim() != 3 or query.size(2) != dim or query.size(1) % kv_heads or query.size(1) == 0:
@@ -168,30 +169,27 @@ def _decode(query, k_pool, v_pool, page_table, context_lens, local_window, selec
         raise ValueError("context_lens is required with page_table")
     code = dtype_code(query)
     lens = as_int32(context_lens).contiguous()
-    if table.size(0) != batch or lens.shape != (batch,) or lens.device != dev:
+    if table.size(0) != batch or lens.dim() != 1 or lens.size(0) != batch or lens.get_device() != dev:
         raise ValueError("page_table must be [batch, pages] and context_lens [batch]")
+    w_ptr, w_tokens = None, 0
     if weights is not None:
         check_weights(weights, batch, kv_heads, dev)
+        w_ptr, w_tokens = weights.data_ptr(), weights.size(2)
     tokens = table.size(1) * page
-    top_m = 0
+    top_m, s_ptr = 0, None
     most = min(tokens, local_window) if local_window else tokens
     if selected is not None:
-        top_m = selected.size(1)
+        top_m, s_ptr = selected.size(1), selected.data_ptr()
         most = min(tokens, local_window) + top_m * page
     out = torch.empty_like(query)
     if batch == 0:
         return out
-    need = _lib.lib.spa_cache_decode_workspace_size(batch, q_heads, kv_heads, dim, most, tokens, weights is not None,
-                                                    -1)
+    need = _lib.lib.spa_cache_decode_workspace_size(batch, q_heads, kv_heads, dim, most, tokens, w_ptr is not None, -1)
     # from the caching allocator, per call: ordered with the stream, and a captured graph keeps its own
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    with on_device(dev):
-        rc = _lib.lib.spa_int4_decode(
-            query.data_ptr(), code, batch, q_heads, kv_heads, dim, ctypes.byref(layout), k_pool[1].data_ptr(),
-            v_pool[1].data_ptr(), lens.data_ptr(), tokens, local_window,
-            selected.data_ptr() if selected is not None else None, top_m, most, dim ** -0.5, out.data_ptr(),
-            weights.data_ptr() if weights is not None else None, weights.size(2) if weights is not None else 0,
-            ws.data_ptr() if ws is not None else None, need, stream_ptr(dev))
+    ws = torch.empty(need, dtype=torch.uint8, device=table.device) if need else None
+    rc = launch(_lib.lib.spa_int4_decode, dev, query.data_ptr(), code, batch, q_heads, kv_heads, dim,
+                ctypes.byref(layout), k_scales, v_scales, lens.data_ptr(), tokens, local_window, s_ptr, top_m, most,
+                dim ** -0.5, out.data_ptr(), w_ptr, w_tokens, ws.data_ptr() if need else None, need)
     _lib.check(rc, "spa_int4_decode")
     return out
 
@@ -217,7 +215,6 @@ def paged_gather_decode_attention_int4(query: torch.Tensor, k_pool, v_pool, sele
         raise ValueError("selected_blocks must be contiguous [batch, top_blocks]")
     if not selected_blocks.is_cuda:
         raise ValueError("contiguous CUDA tensors are required")
-    if selected_blocks.device != query.device:
-        raise ValueError("tensors must be on one device")
+    _same_device(query.get_device(), selected_blocks)
     return _decode(query, k_pool, v_pool, page_table, context_lens, local_window, as_int64(selected_blocks), None,
                    block_size)

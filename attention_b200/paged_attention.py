@@ -22,7 +22,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._util import (as_int32, as_int64, const_i32, dtype_code, on_device, require_contiguous, require_cuda,
+from ._util import (as_int32, as_int64, const_i32, dtype_code, launch, require_contiguous, require_cuda,
                     stream_ptr, workspace)
 from .int4 import check_weights
 
@@ -68,17 +68,15 @@ def _decode(query, kv_layout, kv_heads, context_lens, local_window, selected, to
 
 def _decode_weights(query, layout, kv_heads, lens, tokens, local_window, max_candidates, weights) -> torch.Tensor:
     batch, q_heads, head_dim = query.shape
-    dev = query.device
+    dev = query.get_device()
     check_weights(weights, batch, kv_heads, dev)
     out = torch.empty_like(query)
     code = dtype_code(query)
     need = _lib.lib.spa_cache_decode_workspace_size(batch, q_heads, kv_heads, head_dim, max_candidates, tokens, 1, code)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with on_device(dev):
-        rc = _lib.lib.spa_paged_decode_weights(query.data_ptr(), code, batch, q_heads, kv_heads, head_dim,
-                                               ctypes.byref(layout), lens.data_ptr(), tokens, local_window,
-                                               max_candidates, head_dim ** -0.5, out.data_ptr(), weights.data_ptr(),
-                                               weights.size(2), ws.data_ptr(), need, stream_ptr(dev))
+    ws = torch.empty(need, dtype=torch.uint8, device=query.device)
+    rc = launch(_lib.lib.spa_paged_decode_weights, dev, query.data_ptr(), code, batch, q_heads, kv_heads, head_dim,
+                ctypes.byref(layout), lens.data_ptr(), tokens, local_window, max_candidates, head_dim ** -0.5,
+                out.data_ptr(), weights.data_ptr(), weights.size(2), ws.data_ptr(), need)
     _lib.check(rc, "spa_paged_decode_weights")
     return out
 
