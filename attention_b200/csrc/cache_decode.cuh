@@ -135,13 +135,13 @@ __global__ void __launch_bounds__(kPlainWarps * 32) cache_decode_plain_kernel(co
 // ---------------------------------------------------------------------------
 // Joins the partials and, with weights, adds every token's probabilities to its weight.
 // Grid (head blocks + token blocks, Hkv, B): a warp of the first blocks merges one head's output.
-constexpr int kFinishThreads = 256, kFinishTokens = 1024, kFinishHeads = kFinishThreads / 32;
+constexpr int kFinishThreads = 256, kFinishTokens = 2048, kFinishHeads = kFinishThreads / 32;
 
 template <int TILE>
 __global__ void __launch_bounds__(kFinishThreads) cache_decode_finish_kernel(const CacheDecodeArgs a) {
   const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int pairs = a.Hkv * a.chunks, head_blocks = (a.group + kFinishHeads - 1) / kFinishHeads;
-  __shared__ float s_lse[256];
+  __shared__ __align__(16) float s_lse[256];
   __shared__ int s_sum[kFinishThreads / 32][2];
   // this sequence's tiles, those before it, and all
   const TilePlan plan = tile_plan<TILE>(a, b);
@@ -237,15 +237,43 @@ __global__ void __launch_bounds__(kFinishThreads) cache_decode_finish_kernel(con
   }
   __syncthreads();
   const int64_t bh = static_cast<int64_t>(b) * a.Hkv + h;
-  for (int t = t0 + tid; t < min(t0 + kFinishTokens, plan.ctx); t += kFinishThreads) {
-    if (t >= a.T) {
-      spa_raise(SPA_DEVERR_BAD_INDEX);
-      continue;
+  const int t1 = min(t0 + kFinishTokens, min(plan.ctx, a.T));
+  if (tid == 0 && min(t0 + kFinishTokens, plan.ctx) > a.T) spa_raise(SPA_DEVERR_BAD_INDEX);
+  const float* scores = a.scores + bh * a.cap * a.group;
+  float* weights = a.weights + bh * a.T;
+  // kEach tokens a thread, their loads in flight together; the heads in fours where they line up
+  constexpr int kEach = kFinishTokens / kFinishThreads;
+  float w[kEach] = {}, old[kEach] = {};
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (t0 + tid + i * kFinishThreads < t1) old[i] = weights[t0 + tid + i * kFinishThreads];
+  if (a.group % 4 == 0) {
+    for (int n = 0; n < a.group; n += 4) {
+      const float4 lse = *reinterpret_cast<const float4*>(s_lse + n);
+      float4 x[kEach];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int t = min(t0 + tid + i * kFinishThreads, t1 - 1);
+        if (t >= t0) x[i] = *reinterpret_cast<const float4*>(scores + static_cast<int64_t>(t) * a.group + n);
+      }
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        w[i] += fast_exp2(x[i].x - lse.x) + fast_exp2(x[i].y - lse.y) + (fast_exp2(x[i].z - lse.z) + fast_exp2(x[i].w - lse.w));
     }
-    const float* s = a.scores + (bh * a.cap + t) * a.group;
-    float w = 0.f;
-    for (int n = 0; n < a.group; ++n) w += exp2f(s[n] - s_lse[n]);
-    a.weights[bh * a.T + t] += w;
+  } else {
+    for (int n = 0; n < a.group; ++n) {
+      const float lse = s_lse[n];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int t = t0 + tid + i * kFinishThreads;
+        if (t < t1) w[i] += fast_exp2(scores[static_cast<int64_t>(t) * a.group + n] - lse);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int t = t0 + tid + i * kFinishThreads;
+    if (t < t1) weights[t] = old[i] + w[i];
   }
 }
 

@@ -471,16 +471,27 @@ __global__ void __launch_bounds__(Int4Cfg<G, NT>::kWarps * 32, Int4Cfg<G, NT>::k
             if (!(live >> (hh * 16 + g + (e < 2 ? 0 : 8)) & 1)) sc[hh][n][e] = -INFINITY;
     }
     if (a.scores) {
+      // [token][head of the group]; a lane's two heads lie on end
+      const int64_t at = (static_cast<int64_t>(b) * a.Hkv + h) * a.cap;
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int e = 0; e < 4; e += 2) {
+          const int tok = plan.seg + (first_tile + done) * S::kTok + hh * 16 + g + 4 * e;
+          if (tok < plan.lo || tok >= plan.ctx) continue;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int tok = plan.seg + (first_tile + done) * S::kTok + hh * 16 + g + (e < 2 ? 0 : 8), head = n * 8 + 2 * t + (e & 1);
-            if (tok >= plan.lo && tok < plan.ctx && head < heads)
-              a.scores[((static_cast<int64_t>(b) * a.Hkv + h) * a.cap + tok) * a.group + head0 + head] = sc[hh][n][e] * q_unit[n][e & 1];
+          for (int n = 0; n < NT; ++n) {
+            const int head = n * 8 + 2 * t;
+            float* p = a.scores + (at + tok) * a.group + head0 + head;
+            const float x = sc[hh][n][e] * q_unit[n][0], y = sc[hh][n][e + 1] * q_unit[n][1];
+            if (head + 1 < heads && a.group % 2 == 0) {
+              *reinterpret_cast<float2*>(p) = make_float2(x, y);
+            } else if (head < heads) {
+              p[0] = x;
+              if (head + 1 < heads) p[1] = y;
+            }
           }
+        }
     }
     // ---- running maximum and sum.  The maximum is only moved once a score passes it by
     // 2^kSlack: until then probabilities reach 2^kSlack instead of 1, for which unit leaves room.

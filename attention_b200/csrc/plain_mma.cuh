@@ -153,8 +153,12 @@ __global__ void __launch_bounds__(PlainCfg<D>::kWarps * 32, PlainCfg<D>::kCtas) 
         const int tk = tok + g + 8 * e;
         if (tk >= plan.lo && tk < plan.ctx) {
           float* p = a.scores + ((static_cast<int64_t>(b) * a.Hkv + h) * a.cap + tk) * a.group + head0 + h0;
-          p[0] = sc[2 * e];
-          if (h0 + 1 < heads) p[1] = sc[2 * e + 1];
+          if (h0 + 1 < heads && a.group % 2 == 0) {
+            *reinterpret_cast<float2*>(p) = make_float2(sc[2 * e], sc[2 * e + 1]);
+          } else {
+            p[0] = sc[2 * e];
+            if (h0 + 1 < heads) p[1] = sc[2 * e + 1];
+          }
         }
       }
     }
