@@ -198,8 +198,9 @@ __global__ void __launch_bounds__(kSelThreads, 4) select_tokens_kernel(const flo
 // behind every row stored so far, so its loads are in flight meanwhile, and the rows of the
 // chunk after that (keep, then the page table) are being looked up, once a row.
 //
-// Bound by HBM (each kept row read and written once).  One CTA a pool and pair leaves that to
-// the latency of its chunks: 64 pairs, 8192 of 32768 rows of 256 bytes took 777 us that way.
+// Bound by HBM (each kept row read and written once) and the cluster's rounds: 64 pairs, 8192 of
+// 32768 rows of 256 bytes take 123 us, 0.69 of the copy bandwidth (777 us with one CTA a pool
+// and pair, 137 with both look-ups of a row in one step).
 constexpr int kMaxPools = 8;
 struct CompactArgs {
   unsigned char* pool[kMaxPools];
@@ -213,21 +214,60 @@ struct CompactArgs {
   int T;
 };
 
-constexpr int kCompactThreads = 256, kCompactUnroll = 4;
+constexpr int kCompactThreads = 256, kCompactUnroll = 4, kCompactCtas = 4;
 
-// Row of token t, or -1 (with the error word set) where it has no page.
-__device__ __forceinline__ int64_t compact_row(const CompactArgs& a, int b, int h, int t) {
-  int lp = static_cast<int>(__umulhi(static_cast<uint32_t>(t), a.page_inv)), off = t - lp * a.addr.page_size;
-  if (off >= a.addr.page_size) ++lp, off -= a.addr.page_size;
-  const int64_t pg = a.addr.page_of(b, lp);
-  const int64_t row =
-      b * a.addr.batch_stride_rows + pg * a.addr.page_stride_rows + h * a.addr.head_stride_rows + off;
-  if (pg < 0 || row < 0 || row >= a.addr.total_rows) {
-    spa_raise(SPA_DEVERR_BAD_PAGE);
-    return -1;
+// The rows that entry j of a list moves between, found in three steps of one load each, so that
+// none waits for the one before: first() the token, second() the pages, third() the rows (to < 0
+// to leave the entry out, with the error word set where a page is missing).  A call of each takes
+// up what the call of the step before it left.
+struct CompactPool {
+  const CompactArgs& a;
+  const int32_t* keep;
+  int b, h;
+  int j = 0, token = -1;
+  int page[2] = {-1, -1}, off[2] = {0, 0};
+  bool go = false;
+
+  __device__ __forceinline__ void first(int entry, bool valid) {
+    j = entry;
+    token = valid ? keep[entry] : -1;
   }
-  return row;
-}
+  __device__ __forceinline__ void second() {
+    go = token >= 0 && token != j;
+    if (!go) return;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int t = e ? j : token;
+      int lp = static_cast<int>(__umulhi(static_cast<uint32_t>(t), a.page_inv));
+      off[e] = t - lp * a.addr.page_size;
+      if (off[e] >= a.addr.page_size) ++lp, off[e] -= a.addr.page_size;
+      page[e] = !a.addr.page_table ? lp
+                : lp < a.addr.table_stride ? a.addr.page_table[static_cast<int64_t>(b) * a.addr.table_stride + lp] : -1;
+    }
+  }
+  __device__ __forceinline__ longlong2 third() const {
+    if (!go) return make_longlong2(-1, -1);
+    int64_t row[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      row[e] = b * a.addr.batch_stride_rows + page[e] * a.addr.page_stride_rows + h * a.addr.head_stride_rows + off[e];
+    if (page[0] < 0 || page[1] < 0 || row[0] < 0 || row[1] < 0 || row[0] >= a.addr.total_rows || row[1] >= a.addr.total_rows) {
+      spa_raise(SPA_DEVERR_BAD_PAGE);
+      return make_longlong2(-1, -1);
+    }
+    return make_longlong2(row[0], row[1]);
+  }
+};
+struct CompactWeights {
+  const int32_t* keep;
+  int j = 0, token = -1, to = -1, from = -1;
+  __device__ __forceinline__ void first(int entry, bool valid) {
+    j = entry;
+    token = valid ? keep[entry] : -1;
+  }
+  __device__ __forceinline__ void second() { from = token, to = token >= 0 ? j : -1; }
+  __device__ __forceinline__ longlong2 third() const { return make_longlong2(from, to); }
+};
 
 // A chunk of a CTA: the fewer of 256 rows and what its threads hold in kCompactUnroll units each.
 __host__ __device__ inline int compact_chunk_rows(int per) {
@@ -237,7 +277,6 @@ __host__ __device__ inline int compact_chunk_rows(int per) {
 
 // rows: of the pair; per: units a row; rank, ranks: of the CTA in its cluster; slot: 4 tables of
 // a chunk's (source, destination) rows, so that a thread may be a chunk ahead of another.
-// at(j, from, to): rows of entry j of the list, to < 0 to leave it out.
 template <typename U, typename At>
 __device__ __forceinline__ void compact_rows(U* pool, int rows, int per, int rank, int ranks,
                                              longlong2 (*slot)[kCompactThreads], At at) {
@@ -250,14 +289,12 @@ __device__ __forceinline__ void compact_rows(U* pool, int rows, int per, int ran
     off_of[u] = i - row_of[u] * per;
     if (row_of[u] >= chunk) row_of[u] = -1;
   }
-  const auto look_up = [&](int c) {
-    if (static_cast<int>(threadIdx.x) < chunk) {
-      const int j = (c * ranks + rank) * chunk + threadIdx.x;
-      int64_t from = -1, to = -1;
-      if (c < chunks && j < rows) at(j, from, to);
-      slot[c & 3][threadIdx.x] = make_longlong2(from, to);
-    }
+  const bool looks = static_cast<int>(threadIdx.x) < chunk;
+  const auto first = [&](int c) {
+    const int j = (c * ranks + rank) * chunk + threadIdx.x;
+    at.first(j, c < chunks && j < rows);
   };
+  const auto write = [&](int c) { slot[c & 3][threadIdx.x] = at.third(); };
   U v[2][kCompactUnroll] = {};
   const auto load = [&](int c, int k) {
 #pragma unroll
@@ -291,14 +328,26 @@ __device__ __forceinline__ void compact_rows(U* pool, int rows, int per, int ran
     }
     cluster_arrive_relaxed();
   };
-  look_up(0);
-  look_up(1);
+  if (looks) {
+    for (int c = 0; c < 2; ++c) {
+      first(c);
+      at.second();
+      write(c);
+    }
+    first(2);
+    at.second();
+    first(3);
+  }
   __syncthreads();
   load(0, 0);
   for (int c = 0; c < chunks; c += 2) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      look_up(c + k + 2);
+      if (looks) {
+        write(c + k + 2);
+        at.second();
+        first(c + k + 4);
+      }
       arrive(k);
       if (c + k + 1 < chunks) load(c + k + 1, 1 - k);
       cluster_wait();
@@ -308,7 +357,7 @@ __device__ __forceinline__ void compact_rows(U* pool, int rows, int per, int ran
   }
 }
 
-__global__ void __launch_bounds__(kCompactThreads, 4) compact_kernel(const CompactArgs a) {
+__global__ void __launch_bounds__(kCompactThreads, kCompactCtas) compact_kernel(const CompactArgs a) {
   uint32_t rank, ranks;
   asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
   asm volatile("mov.u32 %0, %cluster_nctarank;" : "=r"(ranks));
@@ -350,12 +399,7 @@ __global__ void __launch_bounds__(kCompactThreads, 4) compact_kernel(const Compa
     unsigned char* pool = a.pool[which];
     const int bytes = a.row_bytes[which];
     // a row whose source or destination has no page is left out whole
-    const auto at = [&](int j, int64_t& from, int64_t& to) {
-      const int k = keep[j];
-      if (k == j) return;
-      from = compact_row(a, b, h, k);
-      if (from >= 0) to = compact_row(a, b, h, j);
-    };
+    const CompactPool at{a, keep, b, h};
     switch (a.unit[which]) {
       case 16: compact_rows(reinterpret_cast<uint4*>(pool), n, bytes / 16, rank, ranks, s_rows, at); break;
       case 8: compact_rows(reinterpret_cast<uint2*>(pool), n, bytes / 8, rank, ranks, s_rows, at); break;
@@ -363,12 +407,10 @@ __global__ void __launch_bounds__(kCompactThreads, 4) compact_kernel(const Compa
       case 2: compact_rows(reinterpret_cast<uint16_t*>(pool), n, bytes / 2, rank, ranks, s_rows, at); break;
       default: compact_rows(pool, n, bytes, rank, ranks, s_rows, at); break;
     }
-  } else if (a.weights) {
+  }
+  if (which == 0 && a.weights) {
     float* w = a.weights + bh * a.T;
-    compact_rows(reinterpret_cast<uint32_t*>(w), n, 1, rank, ranks, s_rows, [&](int j, int64_t& from, int64_t& to) {
-      from = keep[j];
-      to = j;
-    });
+    compact_rows(reinterpret_cast<uint32_t*>(w), n, 1, rank, ranks, s_rows, CompactWeights{keep});
     // the sources behind row n have all been loaded (an empty list had no chunk to wait for,
     // and no sources)
     for (int t = n + rank * kCompactThreads + threadIdx.x; t < a.T; t += ranks * kCompactThreads) w[t] = 0.f;
@@ -420,7 +462,9 @@ extern "C" int spa_compact_tokens(const spa_kv_layout* kv, int n_pools, void* co
   a.budget = budget;
   a.weights = weights;
   a.T = weight_tokens;
-  // CTAs a cluster: as many as have a chunk of some pool's rows, up to the portable 8
+  // CTAs a cluster: as many as have a chunk of some pool's rows, up to the portable 8, and no more
+  // than the GPU holds at once (kCompactCtas an SM): 64 pairs' K and V of 8192 rows took 143 us
+  // in clusters of 8, 137 in clusters of 4
   int64_t most = weights ? (budget + spa::kCompactThreads - 1) / spa::kCompactThreads : 1;
   for (int i = 0; i < n_pools; ++i) {
     const int per = row_bytes[i] / a.unit[i];
@@ -428,8 +472,11 @@ extern "C" int spa_compact_tokens(const spa_kv_layout* kv, int n_pools, void* co
     const int64_t chunks = (budget + spa::compact_chunk_rows(per) - 1) / spa::compact_chunk_rows(per);
     most = chunks > most ? chunks : most;
   }
+  const int planes = n_pools > 0 ? n_pools : 1;
+  const int64_t room = static_cast<int64_t>(spa::device_sm_count()) * spa::kCompactCtas / (static_cast<int64_t>(batch) * kv_heads * planes);
+  if (room < most) most = room;
   const int ranks = most >= 8 ? 8 : most >= 4 ? 4 : most >= 2 ? 2 : 1;
-  SPA_CHECK_CUDA(spa::launch_ex(spa::compact_kernel, dim3((n_pools + (weights ? 1 : 0)) * ranks, kv_heads, batch),
-                                dim3(spa::kCompactThreads), 0, reinterpret_cast<cudaStream_t>(stream), false, ranks, a));
+  SPA_CHECK_CUDA(spa::launch_ex(spa::compact_kernel, dim3(planes * ranks, kv_heads, batch), dim3(spa::kCompactThreads), 0,
+                                reinterpret_cast<cudaStream_t>(stream), false, ranks, a));
   return SPA_OK;
 }
