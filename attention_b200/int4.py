@@ -15,6 +15,7 @@ the pools (page summaries for the router come from the keys before they are appe
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -152,6 +153,12 @@ def check_weights(weights, batch: int, kv_heads: int, dev: int) -> None:
         raise ValueError("weights must be a contiguous float32 tensor [batch, kv_heads, tokens] on the query's device")
 
 
+@functools.lru_cache(maxsize=256)
+def cache_decode_workspace(*shape) -> int:
+    """``spa_cache_decode_workspace_size``, a function of the shape alone."""
+    return _lib.lib.spa_cache_decode_workspace_size(*shape)
+
+
 def _decode(query, k_pool, v_pool, page_table, context_lens, local_window, selected, weights, block_size=None):
     layout, k_scales, v_scales, kv_heads, dim, table, dev = _pools(k_pool, v_pool, page_table)
     page = layout.page_size
@@ -184,7 +191,7 @@ def _decode(query, k_pool, v_pool, page_table, context_lens, local_window, selec
     out = torch.empty_like(query)
     if batch == 0:
         return out
-    need = _lib.lib.spa_cache_decode_workspace_size(batch, q_heads, kv_heads, dim, most, tokens, w_ptr is not None, -1)
+    need = cache_decode_workspace(batch, q_heads, kv_heads, dim, most, tokens, w_ptr is not None, -1)
     # from the caching allocator, per call: ordered with the stream, and a captured graph keeps its own
     ws = torch.empty(need, dtype=torch.uint8, device=table.device) if need else None
     rc = launch(_lib.lib.spa_int4_decode, dev, query.data_ptr(), code, batch, q_heads, kv_heads, dim,

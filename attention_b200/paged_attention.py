@@ -24,7 +24,7 @@ import torch
 from . import _lib
 from ._util import (as_int32, as_int64, const_i32, dtype_code, launch, require_contiguous, require_cuda,
                     stream_ptr, workspace)
-from .int4 import check_weights
+from .int4 import cache_decode_workspace, check_weights
 
 
 def contiguous_layout(keys: torch.Tensor, values: torch.Tensor, page_size: int) -> _lib.KvLayout:
@@ -72,7 +72,7 @@ def _decode_weights(query, layout, kv_heads, lens, tokens, local_window, max_can
     check_weights(weights, batch, kv_heads, dev)
     out = torch.empty_like(query)
     code = dtype_code(query)
-    need = _lib.lib.spa_cache_decode_workspace_size(batch, q_heads, kv_heads, head_dim, max_candidates, tokens, 1, code)
+    need = cache_decode_workspace(batch, q_heads, kv_heads, head_dim, max_candidates, tokens, 1, code)
     ws = torch.empty(need, dtype=torch.uint8, device=query.device)
     rc = launch(_lib.lib.spa_paged_decode_weights, dev, query.data_ptr(), code, batch, q_heads, kv_heads, head_dim,
                 ctypes.byref(layout), lens.data_ptr(), tokens, local_window, max_candidates, head_dim ** -0.5,
