@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kPlainWarps * 32) cache_decode_plain_kernel(co
 // Grid (head blocks + token blocks, Hkv, B): a warp of the first blocks merges one head's output.
 constexpr int kFinishThreads = 256, kFinishTokens = 2048, kFinishHeads = kFinishThreads / 32;
 
-template <int TILE>
+template <int TILE, bool WEIGHTS>
 __global__ void __launch_bounds__(kFinishThreads) cache_decode_finish_kernel(const CacheDecodeArgs a) {
   const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int pairs = a.Hkv * a.chunks, head_blocks = (a.group + kFinishHeads - 1) / kFinishHeads;
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kFinishThreads) cache_decode_finish_kernel(con
     if (a.ctas)
       ctas_of(before * pairs + static_cast<int64_t>(hc) * plan.n, plan.n, total * pairs, a.ctas, first, last);
     first += pair, last += pair;
-    if (first == last && !a.weights) return 0.f;  // its CTA has written the output
+    if (first == last && !WEIGHTS) return 0.f;  // its CTA has written the output
     float M = -INFINITY;
     for (int s = first + lane; s <= last; s += 32) M = fmaxf(M, a.part_lse[static_cast<int64_t>(s) * a.heads + row]);
 #pragma unroll
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kFinishThreads) cache_decode_finish_kernel(con
       return;
     }
     const float lse = lse_of(n);
-    if (first == last && !a.weights) return;
+    if (first == last && !WEIGHTS) return;
     // eight partials' loads in flight; four columns a lane where rows allow
     const auto columns = [&](auto vec) {
       constexpr int V = decltype(vec)::value;
@@ -229,6 +229,7 @@ __global__ void __launch_bounds__(kFinishThreads) cache_decode_finish_kernel(con
       columns(std::integral_constant<int, 1>{});
     return;
   }
+  if constexpr (!WEIGHTS) return;
   const int t0 = plan.lo + (blockIdx.x - head_blocks) * kFinishTokens;
   if (t0 >= plan.ctx) return;
   for (int n = warp; n < a.group; n += kFinishThreads / 32) {
@@ -383,8 +384,10 @@ int cache_decode_impl(CacheDecodeArgs a, int kv_dtype, const spa_kv_layout* kv, 
   if (rc || !parts) return rc;
   const int span = a.local_window > 0 && a.local_window < a.cap ? a.local_window : a.cap;
   const int blocks = (a.group + kFinishHeads - 1) / kFinishHeads + (a.weights ? (span + kFinishTokens - 1) / kFinishTokens : 0);
-  SPA_CHECK_CUDA(launch_pdl(p.tile == 16 ? cache_decode_finish_kernel<16> : cache_decode_finish_kernel<32>,
-                            dim3(blocks, a.Hkv, a.B), dim3(kFinishThreads), 0, st, true, a));
+  // (without weights every path has tiles of 32)
+  auto finish = !a.weights ? cache_decode_finish_kernel<32, false>
+                : p.tile == 16 ? cache_decode_finish_kernel<16, true> : cache_decode_finish_kernel<32, true>;
+  SPA_CHECK_CUDA(launch_pdl(finish, dim3(blocks, a.Hkv, a.B), dim3(kFinishThreads), 0, st, true, a));
   return SPA_OK;
 }
 

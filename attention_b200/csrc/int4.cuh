@@ -139,7 +139,7 @@ __device__ __forceinline__ void quantise_group(const float (&x)[32], uint32_t (&
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kInt4Warps * 32, 6) int4_append_kernel(const Int4Rows a, const T* __restrict__ k_new,
+__global__ void __launch_bounds__(kInt4Warps * 32, 5) int4_append_kernel(const Int4Rows a, const T* __restrict__ k_new,
                                                                       const T* __restrict__ v_new, int64_t sb,
                                                                       int64_t sh, int64_t st, int vec) {
   __shared__ __align__(16) uint16_t s_words[kInt4Warps][256];

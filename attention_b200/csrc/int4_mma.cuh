@@ -167,9 +167,9 @@ __device__ __forceinline__ void nibbles(uint32_t x, uint32_t (&n)[4]) {
     n[3] = x & 0x00f000f0u;
   }
 }
-// z + 8 s of two fp16 pairs as a sum of two halves each
-__device__ __forceinline__ void centre_zero(uint32_t& z, uint32_t& low, uint32_t s) {
-  const float a = fmaf(8.f, half_lo(s), half_lo(z)), b = fmaf(8.f, half_hi(s), half_hi(z));
+// z + 8 s of two fp16 pairs, times `unit`, as a sum of two halves each
+__device__ __forceinline__ void centre_zero(uint32_t& z, uint32_t& low, uint32_t s, float unit) {
+  const float a = fmaf(8.f, half_lo(s), half_lo(z)) * unit, b = fmaf(8.f, half_hi(s), half_hi(z)) * unit;
   z = pack_h2(a, b);
   low = pack_h2(a - half_lo(z), b - half_hi(z));
 }
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(Int4Cfg<G, NT>::kWarps * 32, Int4Cfg<G, NT>::k
   __shared__ int pre[kFlatBatch + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   unsigned char* ring = i4_smem + warp * (ST * S::kStage);
-  pdl_trigger();
+  if (a.ctas || a.weights) pdl_trigger();  // the kernel that joins the partials comes next
   if (a.ctas) tiles_before<S::kTok>(a, pre);
   Work work(a, pre);
   Segment seg;
@@ -383,6 +383,10 @@ __global__ void __launch_bounds__(Int4Cfg<G, NT>::kWarps * 32, Int4Cfg<G, NT>::k
   // halves of those, over the widest range.
   uint32_t top = 0x3c00u;
   float unit2 = kUnit2;
+  // z + 8 s is held as it is, or, once scales above kWide = 4096 turned up (it might pass fp16's
+  // range), in sixteenths
+  constexpr uint32_t kWide = 0x6c00u;
+  float z_unit = 1.f;
 
   int stage = 0;
 #pragma unroll 1
@@ -396,6 +400,14 @@ __global__ void __launch_bounds__(Int4Cfg<G, NT>::kWarps * 32, Int4Cfg<G, NT>::k
     const unsigned char* vsc = ksc + S::kScales;
     const unsigned live = s_live[warp][stage];
     float sc[2][NT][4], mn[NT][2];
+    float zk_unit = 1.f;  // as z_unit, for this tile of K
+    if constexpr (kCentreK) {
+      uint32_t ktop[(G + 1) / 2], most = 0;
+      lds_words<2 * G>(ksc + lane * S::kScaleRow, ktop);
+#pragma unroll
+      for (int i = 0; i < (G + 1) / 2; ++i) most = __vmaxu2(most, ktop[i]);
+      if (__any_sync(0xffffffffu, max(most & 0xffffu, most >> 16) > kWide)) zk_unit = 0.0625f;
+    }
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
       const int r0 = hh * 16 + g, r1 = r0 + 8;
@@ -421,8 +433,8 @@ __global__ void __launch_bounds__(Int4Cfg<G, NT>::kWarps * 32, Int4Cfg<G, NT>::k
       };
       uint32_t z0 = pair_at(r0, G), z1 = pair_at(r1, G), zl0 = 0, zl1 = 0;
       if constexpr (kCentreK) {
-        centre_zero(z0, zl0, pair_at(r0, 0));
-        centre_zero(z1, zl1, pair_at(r1, 0));
+        centre_zero(z0, zl0, pair_at(r0, 0), zk_unit);
+        centre_zero(z1, zl1, pair_at(r1, 0), zk_unit);
       }
       float acc[NT][4];
 #pragma unroll
@@ -458,7 +470,7 @@ __global__ void __launch_bounds__(Int4Cfg<G, NT>::kWarps * 32, Int4Cfg<G, NT>::k
         mma_f16_zero(c, z0, z1, z0, z1, qz[n][0], qz[n][1]);
         if constexpr (kCentreK) mma_f16(c, zl0, zl1, zl0, zl1, qz[n][0], qz[n][1]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[hh][n][e] = fmaf(acc[n][e], kUnitK, c[e]);
+        for (int e = 0; e < 4; ++e) sc[hh][n][e] = kCentreK ? fmaf(c[e], 1.f / zk_unit, acc[n][e]) : fmaf(acc[n][e], kUnitK, c[e]);
       }
     }
     if (live != 0xffffffffu) {
@@ -516,6 +528,13 @@ __global__ void __launch_bounds__(Int4Cfg<G, NT>::kWarps * 32, Int4Cfg<G, NT>::k
         const uint32_t to = (all + 0x3ffu) & 0x7c00u;  // the next power of two
         shrink = __uint_as_float((127u - ((to - top) >> 10)) << 23);
         unit2 -= static_cast<float>((to - top) >> 10);
+        if (to > kWide && top <= kWide) {
+          z_unit = 0.0625f;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) zo[n][e] *= z_unit;
+        }
         top = to;
       }
 #pragma unroll
@@ -581,11 +600,12 @@ __global__ void __launch_bounds__(Int4Cfg<G, NT>::kWarps * 32, Int4Cfg<G, NT>::k
         uint32_t zb = __byte_perm(x[G + 8 * kNext], x[G + 9 * kNext], 0x5410), lb = 0;
         const uint32_t ta = __byte_perm(x[0], x[kNext], 0x5410), tb = __byte_perm(x[8 * kNext], x[9 * kNext], 0x5410);
         if constexpr (PREC > 0) {
-          centre_zero(za, la, ta);
-          centre_zero(zb, lb, tb);
+          centre_zero(za, la, ta, z_unit);
+          centre_zero(zb, lb, tb, z_unit);
         } else {
-          za = hfma2_u(ta, 0x48004800u, za);
-          zb = hfma2_u(tb, 0x48004800u, zb);
+          const uint32_t one = z_unit == 1.f ? 0x3c003c00u : 0x2c002c00u, eight = z_unit == 1.f ? 0x48004800u : 0x38003800u;
+          za = hfma2_u(ta, eight, hmul2_u(za, one));
+          zb = hfma2_u(tb, eight, hmul2_u(zb, one));
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -651,7 +671,7 @@ __global__ void __launch_bounds__(Int4Cfg<G, NT>::kWarps * 32, Int4Cfg<G, NT>::k
       if (g == 0) row[D] = m[n][c] == -INFINITY ? -INFINITY : m[n][c] * q_unit[n][c], row[D + 1] = s * one;
 #pragma unroll
       for (int j = 0; j < G; ++j) {
-        const float z = __shfl_sync(0xffffffffu, zo[n][c] + zo[n][2 + c], j * 4 + t);
+        const float z = __shfl_sync(0xffffffffu, zo[n][c] + zo[n][2 + c], j * 4 + t) * (1.f / z_unit);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
           *reinterpret_cast<float2*>(row + 32 * j + 4 * g + 2 * u) =

@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(PlainCfg<D>::kWarps * 32, PlainCfg<D>::kCtas) 
   __shared__ int pre[kFlatBatch + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   unsigned char* ring = i4_smem + warp * (ST * S::kStage);
-  pdl_trigger();
+  pdl_trigger();  // the kernel that joins the partials comes next
   if (a.ctas) tiles_before<S::kTok>(a, pre);
   Work work(a, pre);
   Segment seg;

@@ -101,7 +101,8 @@ def kv_append_int4(k_pool, v_pool, page_table: torch.Tensor, k_new: torch.Tensor
                    positions: torch.Tensor, *, new_lens: torch.Tensor | None = None) -> None:
     """Quantises ``k_new``/``v_new`` ``[B, Hkv, D]`` (one token) or ``[B, Hkv, T, D]`` into the
     tokens from ``positions[b]`` on; with ``new_lens`` only the first ``new_lens[b]`` of the T.
-    The new tensors may be views with any strides over B, Hkv and T (both the same)."""
+    The new tensors may be views with any strides over B, Hkv and T (both the same).  Tokens
+    before 0 are skipped; no two sequences may write one row."""
     layout, k_scales, v_scales, kv_heads, dim, table, dev = _pools(k_pool, v_pool, page_table)
     batch = table.size(0)
     _same_device(dev, k_new, v_new, positions)

@@ -66,10 +66,13 @@ def _decode(query, kv_layout, kv_heads, context_lens, local_window, selected, to
     return out
 
 
-def _decode_weights(query, layout, kv_heads, lens, tokens, local_window, max_candidates, weights) -> torch.Tensor:
+def _decode_weights(query, layout, kv_heads, lens, tokens, local_window, max_candidates, weights,
+                    borrowed) -> torch.Tensor:
     batch, q_heads, head_dim = query.shape
     dev = query.get_device()
     check_weights(weights, batch, kv_heads, dev)
+    if any(t.get_device() != dev for t in borrowed):
+        raise ValueError("tensors must be on one device")
     out = torch.empty_like(query)
     code = dtype_code(query)
     need = cache_decode_workspace(batch, q_heads, kv_heads, head_dim, max_candidates, tokens, 1, code)
@@ -114,7 +117,8 @@ def paged_decode_attention(query: torch.Tensor, keys: torch.Tensor, values: torc
         lens = const_i32(query.device, batch, length)
         max_cand = length if local_window <= 0 else min(length, local_window)
         if weights is not None:
-            return _decode_weights(query, layout, keys.size(1), lens, length, local_window, max_cand, weights)
+            return _decode_weights(query, layout, keys.size(1), lens, length, local_window, max_cand, weights,
+                                   (keys, values))
         return _decode(query, layout, keys.size(1), lens, local_window, None, 0, max_cand, None)
     if context_lens is None:
         raise ValueError("context_lens is required with page_table")
@@ -129,7 +133,7 @@ def paged_decode_attention(query: torch.Tensor, keys: torch.Tensor, values: torc
         max_cand = min(max_cand, local_window)
     if weights is not None:
         return _decode_weights(query, layout, keys.size(1), lens, table.size(1) * keys.size(2), local_window, max_cand,
-                               weights)
+                               weights, (keys, values, table, lens))
     return _decode(query, layout, keys.size(1), lens, local_window, None, 0, max_cand, (table, lens))
 
 

@@ -751,9 +751,10 @@ int spa_decoder_step(const spa_decoder_step_params* params, spa_stream_t stream)
  * spa_int4_append writes tokens positions[b] + t, t < (new_lens ? new_lens[b] : tokens), from
  * k_new / v_new, whose element (b, h, t, d) lies at b * stride_b + h * stride_h +
  * t * stride_t + d.  A sequence's negative tokens are skipped; a token without a page is
- * skipped and raises device error bit 2.
+ * skipped and raises device error bit 2.  No two sequences may write one row.
  * spa_int4_read writes the same tokens' values to k_out / v_out [B, Hkv, tokens, D]: zeros
- * past lens[b] and where spa_int4_append would have skipped the token.
+ * past lens[b] and where spa_int4_append would have skipped the token (k_out and v_out
+ * 16-byte aligned).
  * No reference counterpart (the reference keeps K/V in the model's dtype).
  */
 int spa_int4_append(const spa_kv_layout* kv, void* k_scales, void* v_scales, int dtype, int batch, int kv_heads,
@@ -780,7 +781,7 @@ int spa_int4_read(const spa_kv_layout* kv, const void* k_scales, const void* v_s
  *
  * Workspace: spa_cache_decode_workspace_size bytes, 16-byte aligned, with any contents; its
  * kv_dtype is the plain cache's, or -1 for the 4-bit cache.  Calls that may overlap need
- * workspaces of their own.  At most 256 query heads per kv head.
+ * workspaces of their own.  At most 256 query heads per kv head; scale is positive.
  */
 size_t spa_cache_decode_workspace_size(int batch, int q_heads, int kv_heads, int head_dim, int max_candidates,
                                        int max_tokens, int weights, int kv_dtype);
@@ -799,7 +800,7 @@ int spa_paged_decode_weights(const void* q, int dtype, int batch, int q_heads, i
  * [batch, kv_heads, tokens].  With L = min(lens[b], tokens): all of them while L <= budget;
  * else the last min(recent, budget) and, of the others, those of the largest weight, ties to
  * the lower token (a NaN is below every number).  keep [batch, kv_heads, budget] holds them in
- * ascending order, then -1; kept_lens[b] = min(L, budget).
+ * ascending order, then -1; kept_lens[b] = min(L, budget) (kept_lens must not overlap lens).
  *
  * spa_compact_tokens: moves row keep[j] to token j, j = 0, 1, ..., in place, in each of the
  * n_pools (up to 8) pools; row_bytes[i] is the size of a row of pools[i], addressed by kv's

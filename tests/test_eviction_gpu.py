@@ -119,6 +119,20 @@ def test_select_tokens(tokens, budget, recent):
     assert torch.equal(keep.cpu(), want) and torch.equal(kept.cpu(), want_kept)
 
 
+@pytest.mark.parametrize("tokens", [300_000, 400_000])
+def test_select_long_rows(tokens):
+    """Rows that just stay in shared memory, and rows that do not."""
+    gen = torch.Generator(device=DEV).manual_seed(tokens)
+    w = torch.rand(1, 2, tokens, generator=gen, device=DEV)
+    w[:, 1] = (w[:, 1] * 50).floor()
+    budget, recent = 70_000, 1000
+    keep, kept = spa.select_tokens(w, torch.tensor([tokens], device=DEV), budget=budget, recent=recent)
+    key = w.clone()
+    key[..., tokens - recent:] = 1e9
+    order = torch.sort(key, dim=2, descending=True, stable=True).indices[..., :budget]
+    assert torch.equal(keep, order.sort(2).values.int()) and kept.item() == budget
+
+
 def test_select_lengths_outside_the_tensor():
     w = torch.rand(3, 2, 50)
     lens = [0, -4, 1000]

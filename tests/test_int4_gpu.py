@@ -207,6 +207,30 @@ def test_decode_small_and_large_values(dtype, scale):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("late", [False, True])
+def test_decode_values_past_fp16(dtype, late):
+    """Ranges whose middle (zero + 8 scales) fp16 could not hold: values of 0 to 2e5, in all tokens or
+    in the last only.  (16-bit outputs: bf16 alone has the range.)"""
+    gen = torch.Generator().manual_seed(17)
+    k, v, table, _, _, _ = make_cache(1, 2, 16, 64, 400, gen)
+    x = torch.rand(2, 1, 2, 400, 64, generator=gen) * 2e5
+    if late:
+        x[..., :390, :] /= 1e5
+    full = [ref.int4_quantise(y) for y in x]
+    for pool, (codes, scales) in zip((k, v), full):
+        for g in range(25):
+            pool[0][table[0, g]] = codes[0, :, g * 16:(g + 1) * 16]
+            pool[1][table[0, g]] = scales[0, :, g * 16:(g + 1) * 16]
+    kval, vval = (ref.int4_dequantise(f) for f in full)
+    q = (torch.randn(1, 4, 64, generator=gen) / 1e5).to(dtype)
+    tokens = [torch.arange(400)]
+    out = spa.paged_decode_attention_int4(q.to(DEV), to_dev(k), to_dev(v), page_table=table.to(DEV),
+                                          context_lens=torch.tensor([400], device=DEV))
+    want, _ = ref.attention_weights(q, kval, vval, tokens)
+    check_out(out, want, bounds(q, full[0], kval, vval, tokens, dtype)[1], dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_decode_peaked_and_shifted_scores(dtype):
     """Scores of some hundreds, rising along the sequence, so that every tile moves the maximum."""
     gen = torch.Generator().manual_seed(5)
@@ -339,6 +363,36 @@ def test_side_stream_and_graph_replay():
         fresh = torch.zeros_like(w)
         again = spa.paged_decode_attention_int4(q, kd, vd, page_table=td, context_lens=lens, weights=fresh)
         assert torch.equal(out, again) and torch.equal(w, fresh)
+
+
+@pytest.mark.parametrize("batch,context", [(40, 900), (1100, 300), (700, 20)])
+def test_decode_long_batches(batch, context):
+    """Batches whose lengths are summed up by more than a warp, batches too long for that, and
+    contexts that one CTA takes whole."""
+    gen = torch.Generator().manual_seed(batch)
+    page, pages = 64, -(-context // 64)
+    cache = spa.PagedKVCacheInt4(batch * pages, 1, page, 32, batch=batch, max_pages_per_seq=pages)
+    cache.page_table.copy_(torch.randperm(batch * pages, generator=gen).view(batch, pages).to(torch.int32))
+    lens = (torch.rand(batch, generator=gen) * (context + 1)).int()
+    lens[::7] = 0
+    new = [torch.randn(batch, 1, context, 32, generator=gen).to(DEV) for _ in range(2)]
+    zero = torch.zeros(batch, dtype=torch.int32, device=DEV)
+    spa.kv_append_int4(cache.k, cache.v, cache.page_table, *new, zero, new_lens=lens.to(DEV))
+    q = torch.randn(batch, 2, 32, generator=gen)
+    w = torch.zeros(batch, 1, context, device=DEV)
+    k, v = (x.double() for x in spa.kv_read_int4(cache.k, cache.v, cache.page_table, zero, context, dtype=torch.float32))
+    args = dict(page_table=cache.page_table, context_lens=lens.to(DEV))
+    plain = spa.paged_decode_attention_int4(q.to(DEV), cache.k, cache.v, **args)
+    out = spa.paged_decode_attention_int4(q.to(DEV), cache.k, cache.v, weights=w, **args)
+    there = (torch.arange(context) < lens[:, None]).to(DEV)[:, None]
+    score = (q.to(DEV).double() @ k[:, 0].transpose(1, 2)) / 32 ** 0.5
+    p = torch.nan_to_num(torch.softmax(torch.where(there, score, -torch.inf), -1))
+    want = p @ v[:, 0]
+    # |q| <= 5 and |k| <= 5 of 32 values: Q <= 5 * 15 * 32 / 32 ** 0.5 < 2^9 (|s n| + |z| <= 15); D + 8 = 40
+    rel = 2 * 40 * 2.0 ** -24 * 2 ** 9 + context * 2.0 ** -24 + 2.0 ** -20
+    for o in (plain, out):
+        assert ((o.double() - want).abs() <= rel * 15).all() and (o[lens == 0] == 0).all()
+    assert ((w[:, 0].double() - p.sum(1)).abs() <= rel * p.sum(1)).all()
 
 
 # ---------------------------------------------------------------- refusals
