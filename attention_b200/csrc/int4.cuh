@@ -1,8 +1,8 @@
 // The 4-bit paged cache: row format, append and read-back.
 //
 // A row (D values of one token of one kv head) is cut into G = D / 32 groups.  Of a group
-// with extremes lo and hi:  s = half((hi - lo) / 15), z = half(lo), both saturating, and
-// n = clamp(rint((x - z) / s), 0, 15) with every step an IEEE fp32 operation (n = 0 where
+// with extremes lo and hi:  s = half((hi - lo) * fl(1/15)), z = half(lo), both saturating,
+// and n = clamp(rint((x - z) / s), 0, 15) with every step an IEEE fp32 operation (n = 0 where
 // s = 0; a group with a NaN or an infinity gets s = z = NaN).  It stands for s * n + z.
 //
 // codes  [pages, Hkv, P, D / 2]: value d = 32 j + 4 g + i of a row is nibble i (low bits
@@ -95,7 +95,7 @@ __device__ __forceinline__ void quantise_group(const float (&x)[32], uint32_t (&
 #pragma unroll
   for (int i = 1; i < 32; ++i) lo = min_nan(lo, x[i]), hi = max_nan(hi, x[i]);
   const bool bad = !(fabsf(lo) < INFINITY && fabsf(hi) < INFINITY);  // a NaN or an infinity among them
-  s = __float2half_rn(fminf(__fdiv_rn(__fsub_rn(hi, lo), 15.f), 65504.f));
+  s = __float2half_rn(fminf(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f), 65504.f));
   z = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
   const float sf = __half2float(s), zf = __half2float(z);
   if (bad) s = z = __ushort_as_half(0x7fff);

@@ -24,6 +24,12 @@
 // streams a stretch of tiles of 32 tokens (5 KB) through its own ring of cp.async stages in
 // shared memory, without barriers between warps, so pages of any size, order and alignment
 // cost the same.
+//
+// Measured (B200, 32 query and 8 kv heads of 128, bf16, pages of 128): 8 x 32768 tokens 76 us, 4.4
+// TB/s or 0.67 of the copy bandwidth; 8 x 131072 tokens 259 us, 0.79.  In long contexts what is
+// left is the instructions (IPC 2.3 of 4 with 12 warps an SM; with 16 warps of 128 registers it
+// was 80 us, with the maximum moved at every rise 90); some 12 us of every call are the phases
+// before the first product and after the last, and the joining kernel.
 #pragma once
 
 #include "cache_args.cuh"

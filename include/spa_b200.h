@@ -740,7 +740,8 @@ int spa_decoder_step(const spa_decoder_step_params* params, spa_stream_t stream)
  * The 4-bit paged cache.  Addressing is spa_kv_layout's, its "rows" being codes of
  * head_dim / 2 bytes (k and v point to them); k_scales and v_scales hold 2 * head_dim / 32
  * fp16 per row.  A row is cut into G = head_dim / 32 groups of 32 values.  For a group with
- * extremes lo and hi, in fp32 arithmetic: scale = fp16((hi - lo) / 15), zero = fp16(lo), both
+ * extremes lo and hi, in fp32 arithmetic: scale = fp16((hi - lo) * r) with r the fp32 value next
+ * to 1/15, zero = fp16(lo), both
  * clamped to +-65504; n = clamp(rint((x - zero) / scale), 0, 15), 0 where scale is 0; it
  * stands for scale * n + zero.  A group that holds a NaN or an infinity reads back as NaN.
  *   codes  [pages, Hkv, P, D / 2]  value d = 32 j + 4 g + i is nibble i (low bits first) of

@@ -22,7 +22,7 @@ def int4_quantise(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     scales = np.zeros((a.shape[0], 2, g), np.float16)
     with np.errstate(all="ignore"):
         lo, hi = a.min(-1), a.max(-1)
-        s = np.minimum((hi - lo) / np.float32(15), np.float32(65504)).astype(np.float16)
+        s = np.minimum((hi - lo) * np.float32(1 / 15), np.float32(65504)).astype(np.float16)
         z = np.clip(lo, np.float32(-65504), np.float32(65504)).astype(np.float16)
         n = np.rint((a - z.astype(np.float32)[..., None]) / s.astype(np.float32)[..., None])
     n = np.where((s > 0)[..., None], np.clip(n, 0, 15), 0)
