@@ -84,11 +84,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return y;
 }
 
-// (out of line: the division is rare, and inlined 32 times it costs 40 registers)
-__device__ __noinline__ uint32_t divided_code(float d, float s) {
-  return static_cast<uint32_t>(fminf(fmaxf(rintf(__fdiv_rn(d, s)), 0.f), 15.f));
-}
-
 // A group's 8 words of 4 codes, its scale and zero.
 __device__ __forceinline__ void quantise_group(const float (&x)[32], uint32_t (&word)[8], __half& s, __half& z) {
   float lo = x[0], hi = x[0];
@@ -99,47 +94,27 @@ __device__ __forceinline__ void quantise_group(const float (&x)[32], uint32_t (&
   z = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
   const float sf = __half2float(s), zf = __half2float(z);
   if (bad) s = z = __ushort_as_half(0x7fff);
-  const bool none = bad || !(sf > 0.f);
-  // rint((x - z) / s) by the clamped product with 1 / (15 s): within 4e-6 of the quotient, so
-  // where the product is further than that from a half it rounds to the same code.  Adding
-  // 1.5 2^23 rounds to the integer, ties to even.
-  constexpr float kMagic = 12582912.f, kNear = 0.49999f;
-  const float inv = none ? 0.f : 1.f / (15.f * sf);
-  float off = 0.f;
+  // The quotient by Markstein's theorem (Computation of elementary functions on the IBM RISC
+  // System/6000, 1990): with y the rounded reciprocal of s and q0 = fl(d y), the fused
+  // q0 + (d - q0 s) y is d / s rounded.  Without a scale y = 0 and every code 0 (a NaN as well).
+  // Adding 1.5 2^23 rounds to the integer, ties to even.
+  constexpr float kMagic = 12582912.f;
+  const float y = !bad && sf > 0.f ? __frcp_rn(sf) : 0.f;
 #pragma unroll
   for (int w = 0; w < 8; ++w) {
     float n[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float q = __saturatef(__fsub_rn(x[4 * w + e], zf) * inv);
-      n[e] = fmaf(q, 15.f, kMagic) - kMagic;
-      off = fmaxf(off, fabsf(fmaf(q, 15.f, -n[e])));
+      const float d = __fsub_rn(x[4 * w + e], zf), q0 = __fmul_rn(d, y);
+      const float q = fmaf(fmaf(-q0, sf, d), y, q0);
+      n[e] = __fsub_rn(__fadd_rn(fminf(fmaxf(q, 0.f), 15.f), kMagic), kMagic);
     }
     word[w] = static_cast<uint32_t>(fmaf(n[3], 4096.f, fmaf(n[2], 256.f, fmaf(n[1], 16.f, n[0]))));
-  }
-  // Values next to a half (with 16-bit inputs 1 in 1400: x - z and s have few bits): the division
-  // decides
-  if (off > kNear) {
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float d = __fsub_rn(x[4 * w + e], zf), q = __saturatef(d * inv) * 15.f;
-        if (fabsf(q - rintf(q)) > kNear) {
-          const uint32_t n = divided_code(d, sf);
-          word[w] = (word[w] & ~(15u << (4 * e))) | n << (4 * e);
-        }
-      }
-    }
-  }
-  if (none) {
-#pragma unroll
-    for (int w = 0; w < 8; ++w) word[w] = 0;
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kInt4Warps * 32, 5) int4_append_kernel(const Int4Rows a, const T* __restrict__ k_new,
+__global__ void __launch_bounds__(kInt4Warps * 32) int4_append_kernel(const Int4Rows a, const T* __restrict__ k_new,
                                                                       const T* __restrict__ v_new, int64_t sb,
                                                                       int64_t sh, int64_t st, int vec) {
   __shared__ __align__(16) uint16_t s_words[kInt4Warps][256];
