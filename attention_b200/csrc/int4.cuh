@@ -169,6 +169,10 @@ __global__ void __launch_bounds__(kInt4Warps * 32) int4_read_kernel(const Int4Ro
   const int64_t my_row = t0 + lane < min(t1, len) ? int4_row(a, b, h, t0 + lane, true) : -1;
   const int rows = 32 / a.G, r = lane / a.G, j = lane - r * a.G;
   uint16_t* words = s_words[warp];
+  // words of group j of row r lie at 8 G r + j + G g
+  const int grp0 = lane >> 2, row0 = grp0 / a.G, first_j = grp0 - row0 * a.G;
+  const int first_word = row0 * a.G * 8 + first_j + (lane & 3) * 2 * a.G;
+  const int eight_rows = 8 / a.G, eight_j = 8 - eight_rows * a.G, eight_words = eight_rows * a.G * 8 + eight_j;
   for (int base = 0; base < t1 - t0; base += rows) {
     const int i = base + r;
     const bool in = r < rows && t0 + i < t1;
@@ -185,10 +189,14 @@ __global__ void __launch_bounds__(kInt4Warps * 32) int4_read_kernel(const Int4Ro
     __syncwarp();
     // eight values a lane: words 2 q and 2 q + 1 of a group; the step's rows lie on end in dst
     const int total = min(rows, t1 - t0 - base) * a.G * 4;
+    int at = first_word, jj = first_j;  // word 0 of the lane's group, and the group's number in its row
     for (int o = lane; o < total; o += 32) {
-      const int grp = o >> 2, rr = grp / a.G, jj = grp - rr * a.G, g = (o & 3) * 2;
-      const uint32_t w0 = words[rr * a.G * 8 + g * a.G + jj], w1 = words[rr * a.G * 8 + (g + 1) * a.G + jj];
-      const float2 c = s_scale[warp][grp];
+      const uint32_t w0 = words[at], w1 = words[at + a.G];
+      const float2 c = s_scale[warp][o >> 2];
+      // eight groups on
+      jj += eight_j;
+      at += eight_words;
+      if (jj >= a.G) jj -= a.G, at += a.G * 7;
       // code e of both words at once: under the exponent of 1024 it is the fp16 1024 + n
       T x[8];
       const uint32_t w = w0 | w1 << 16;
