@@ -24,8 +24,8 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // CTA from the number that the CTAs before it hold.
 //
 // Weights are read once and stay in shared memory as keys (longer stretches than that holds are
-// read again).  What bounds it: the latency of those rounds.  64 rows of 32768: 25 us in clusters
-// of 8 (72 us with one CTA a row and the weights read four times; 71, 43 and 29 on the way, with
+// read again).  What bounds it: the latency of those rounds.  64 rows of 32768: 21 us in clusters
+// of 4 (72 us with one CTA a row and the weights read four times; 71, 43 and 29 on the way, with
 // 11-bit digits, with a bin a thread in the search, and with bytes).
 constexpr int kSelThreads = 512, kSelBins = 256, kSelSlice = 4 * kSelThreads;
 constexpr int kSelCached = 40 * 1024;  // keys a CTA keeps
@@ -425,9 +425,17 @@ extern "C" int spa_select_tokens(const float* weights, int batch, int kv_heads, 
   if (!weights || !lens || !keep || !kept_lens || batch <= 0 || batch > 65535 || kv_heads <= 0 || kv_heads > (1 << 20) || tokens <= 0 ||
       budget <= 0 || recent < 0)
     return SPA_ERR_INVALID;
-  // CTAs a cluster: a slice each at least, up to the portable 8
+  // CTAs a cluster: a slice each at least, up to the portable 8; 4 where 8 are more than two CTAs
+  // an SM and 4 fit the GPU at once (64 rows of 32768: 21.1 us against 24.6; of 131072, where they
+  // do not fit: 72.9 against 67.7; 8 rows of 32768: 14.2 against 11.1)
   const int slices = (tokens + spa::kSelSlice - 1) / spa::kSelSlice;
-  const int ranks = slices >= 8 ? 8 : slices >= 4 ? 4 : slices >= 2 ? 2 : 1;
+  int ranks = slices >= 8 ? 8 : slices >= 4 ? 4 : slices >= 2 ? 2 : 1;
+  {
+    const int64_t pairs = static_cast<int64_t>(batch) * kv_heads, sms = spa::device_sm_count();
+    const int64_t bytes = sizeof(uint32_t) * ((static_cast<int64_t>(tokens) + 3) / 4) + 21 * 1024;
+    const int64_t held = 227 * 1024 / bytes < 4 ? 227 * 1024 / bytes : 4;
+    if (ranks == 8 && pairs * 8 > 2 * sms && pairs * 4 <= held * sms) ranks = 4;
+  }
   const int span = (tokens + ranks - 1) / ranks;
   const bool cached = span <= spa::kSelCached;
   const size_t smem = cached ? sizeof(uint32_t) * static_cast<size_t>(span) : 0;
