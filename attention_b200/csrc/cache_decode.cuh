@@ -342,7 +342,7 @@ int cache_decode_impl(CacheDecodeArgs a, int kv_dtype, const spa_kv_layout* kv, 
       max_candidates < 0 || a.cap <= 0 || a.local_window < 0)
     return SPA_ERR_INVALID;
   if (kv->page_size <= 0 || kv->total_rows <= 0 || (kv->page_table && kv->table_stride <= 0)) return SPA_ERR_INVALID;
-  if (!(scale > 0.0) || scale > 1e30) return SPA_ERR_INVALID;
+  if (!(scale > 0.0) || scale > 1e30 || reinterpret_cast<uintptr_t>(a.out) % 16) return SPA_ERR_INVALID;
   if ((a.selected && a.top_m <= 0) || (a.weights && (a.T <= 0 || a.selected))) return SPA_ERR_INVALID;
   a.group = a.Hq / a.Hkv;
   if (a.group > 256) return SPA_ERR_UNSUPPORTED;

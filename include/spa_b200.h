@@ -782,7 +782,8 @@ int spa_int4_read(const spa_kv_layout* kv, const void* k_scales, const void* v_s
  *
  * Workspace: spa_cache_decode_workspace_size bytes, 16-byte aligned, with any contents; its
  * kv_dtype is the plain cache's, or -1 for the 4-bit cache.  Calls that may overlap need
- * workspaces of their own.  At most 256 query heads per kv head; scale is positive.
+ * workspaces of their own.  At most 256 query heads per kv head; scale
+ * is positive, out 16-byte aligned.
  */
 size_t spa_cache_decode_workspace_size(int batch, int q_heads, int kv_heads, int head_dim, int max_candidates,
                                        int max_tokens, int weights, int kv_dtype);

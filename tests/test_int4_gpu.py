@@ -365,6 +365,66 @@ def test_side_stream_and_graph_replay():
         assert torch.equal(out, again) and torch.equal(w, fresh)
 
 
+def test_two_streams_and_two_graphs_at_once():
+    """Calls that run side by side, eagerly and replayed, give what they give alone."""
+    gen = torch.Generator().manual_seed(31)
+    sets = []
+    for i in range(2):
+        k, v, table, _, _, _ = make_cache(3, 2, 32, 128, 2000, gen)
+        lens = torch.tensor([2000, 700 + i, 31], dtype=torch.int32, device=DEV)
+        sets.append((torch.randn(3, 8, 128, generator=gen).to(torch.bfloat16).to(DEV), to_dev(k), to_dev(v),
+                     dict(page_table=table.to(DEV), context_lens=lens), torch.zeros(3, 2, 2000, device=DEV)))
+
+    def step(s, w):
+        w.zero_()
+        return spa.paged_decode_attention_int4(s[0], s[1], s[2], weights=w, **s[3])
+
+    want = [(step(s, s[4]), s[4].clone()) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    graphs = []
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(s, s[4])
+        graphs.append((g, out))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        eager = []
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                w = torch.empty_like(sets[i][4])
+                eager.append((step(sets[i], w), w))
+        torch.cuda.synchronize()
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                graphs[i][0].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(eager[i][0], want[i][0]) and torch.equal(eager[i][1], want[i][1])
+            assert torch.equal(graphs[i][1], want[i][0]) and torch.equal(sets[i][4], want[i][1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_queries_off_16_byte_boundaries(dtype):
+    gen = torch.Generator().manual_seed(6)
+    k, v, table, _, _, _ = make_cache(2, 2, 32, 64, 300, gen)
+    args = (to_dev(k), to_dev(v))
+    more = dict(page_table=table.to(DEV), context_lens=torch.tensor([300, 17], device=DEV))
+    q = torch.randn(2, 8, 64, generator=gen).to(dtype).to(DEV)
+    odd = torch.empty(q.numel() + 1, dtype=dtype, device=DEV)[1:].view(q.shape)
+    odd.copy_(q)
+    assert torch.equal(spa.paged_decode_attention_int4(odd, *args, **more),
+                       spa.paged_decode_attention_int4(q, *args, **more))
+    pool = torch.randn(8, 2, 32, 64, generator=gen).to(dtype).to(DEV)
+    more["page_table"] = torch.arange(8, dtype=torch.int32, device=DEV).view(2, 4)
+    more["context_lens"] = torch.tensor([100, 17], device=DEV)
+    w = [torch.zeros(2, 2, 128, device=DEV) for _ in range(2)]
+    a, b = (spa.paged_decode_attention(x, pool, pool, weights=y, **more) for x, y in zip((odd, q), w))
+    # another kernel may serve the unaligned call: scores of these sizes (Q < 2^6, D + 8 = 72) agree to 2^-10
+    assert ((a - b).abs() <= torch.finfo(dtype).eps * b.abs() + 2.0 ** -10).all()
+    assert ((w[0] - w[1]).abs() <= 2.0 ** -10 * w[1]).all()
+
+
 @pytest.mark.parametrize("batch,context", [(40, 900), (1100, 300), (700, 20)])
 def test_decode_long_batches(batch, context):
     """Batches whose lengths are summed up by more than a warp, batches too long for that, and
