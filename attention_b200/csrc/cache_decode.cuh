@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kFinishThreads) cache_decode_finish_kernel(con
 
 // ---------------------------------------------------------------------------
 // host planning
-constexpr int kWholeTiles = 24, kCtaTiles = 6;
+constexpr int kWholeTiles = 24, kWholeTilesBusy = 40, kCtaTiles = 6;
 enum CacheKernel { kCachePlain, kCacheInt4Mma, kCachePlainMma };
 struct CachePlan {
   int heads, chunks, ctas, slots, tile;
@@ -296,9 +296,12 @@ inline CachePlan cache_plan(int batch, int q_heads, int kv_heads, int head_dim, 
   const int64_t tiles = (max_candidates + p.tile - 1) / p.tile + 1;
   const int64_t room = static_cast<int64_t>(device_sm_count()) * per_sm;
   const int64_t most = (pairs * tiles + kCtaTiles - 1) / kCtaTiles;
-  // One CTA per pair where a pair has little to share, where pairs alone fill the GPU several
-  // times over, or where the batch is longer than a CTA sums up.
-  const bool flat = tiles > kWholeTiles && pairs < 4 * room && batch <= kFlatBatch;
+  // One CTA per pair where a pair has little to share (more of it where pairs alone keep most SMs
+  // busy: 128 pairs of 1000 tokens 12.4 us against 17.3, but of 1800 in fp32 28.4 against 25.5, and 8 of
+  // 1900 in fp16 16.8 against 12.4), where pairs fill the GPU several times over, or where the batch is
+  // longer than a CTA sums up.
+  const bool whole = tiles <= (pairs * 4 >= 3 * device_sm_count() ? kWholeTilesBusy : kWholeTiles);
+  const bool flat = !whole && pairs < 4 * room && batch <= kFlatBatch;
   p.ctas = flat ? static_cast<int>(room < most ? room : most) : 0;
   p.slots = static_cast<int>((flat ? p.ctas : pairs) + pairs);
   return p;

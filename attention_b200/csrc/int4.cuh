@@ -50,8 +50,8 @@ __device__ __forceinline__ int64_t int4_row(const Int4Rows& a, int b, int h, int
 //
 // Bound by HBM (a row's 2 D bytes against its 5/8 D at 16 bits) as long as a value costs few
 // instructions: 9 here to quantise one; with a group spread over 8 lanes and a division a value
-// it was 63.  4 prompts of up to 8192 tokens, 8 heads of 128 in bf16: 77 us for both kernels, 0.54
-// of the copy bandwidth (140 us that way); rows through shared memory by cp.async gave 79.
+// it was 63.  4 prompts of up to 8192 tokens, 8 heads of 128 in bf16: 59 us for both kernels, 0.70
+// of the copy bandwidth (140 us that way).
 constexpr int kInt4Warps = 4, kInt4Stretch = 32;
 
 // 32 consecutive values of a row as fp32; `vec` when 16-byte loads are allowed.
