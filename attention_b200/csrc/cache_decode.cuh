@@ -89,10 +89,11 @@ __global__ void __launch_bounds__(kPlainWarps * 32) cache_decode_plain_kernel(co
       for (int e = 0; e < E; ++e) kv[e] = value(a.v, a.v_scales, row, e);
 #pragma unroll
       for (int n = 0; n < kPlainHeads; ++n) {
-        s[n] *= a.scale_log2;
+        // differences first, then their scale: a scaled score would carry its own rounding
         const float mn = fmaxf(m[n], s[n]);
         // a first score of -inf leaves nothing to weigh: the difference would be NaN
-        const float alpha = m[n] == -INFINITY ? 0.f : exp2f(m[n] - mn), pr = s[n] == -INFINITY ? 0.f : exp2f(s[n] - mn);
+        const float alpha = m[n] == -INFINITY ? 0.f : exp2f((m[n] - mn) * a.scale_log2);
+        const float pr = s[n] == -INFINITY ? 0.f : exp2f((s[n] - mn) * a.scale_log2);
         l[n] = l[n] * alpha + pr;
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[n][e] = fmaf(acc[n][e], alpha, pr * kv[e]);
@@ -100,7 +101,7 @@ __global__ void __launch_bounds__(kPlainWarps * 32) cache_decode_plain_kernel(co
       }
       if (a.scores && lane == 0)
         for (int n = 0; n < heads; ++n)
-          a.scores[((static_cast<int64_t>(b) * a.Hkv + h) * a.cap + t) * a.group + head0 + n] = s[n];
+          a.scores[((static_cast<int64_t>(b) * a.Hkv + h) * a.cap + t) * a.group + head0 + n] = s[n] * a.scale_log2;
     }
   }
   // merge the warps
@@ -116,14 +117,14 @@ __global__ void __launch_bounds__(kPlainWarps * 32) cache_decode_plain_kernel(co
     float M = -INFINITY, W = 0.f, O = 0.f;
     for (int w = 0; w < kPlainWarps; ++w) M = fmaxf(M, sm[w][n]);
     for (int w = 0; w < kPlainWarps; ++w) {
-      const float f = sm[w][n] == -INFINITY ? 0.f : exp2f(sm[w][n] - M);
+      const float f = sm[w][n] == -INFINITY ? 0.f : exp2f((sm[w][n] - M) * a.scale_log2);
       W = fmaf(sl[w][n], f, W);
       O = fmaf(so[w][n][d], f, O);
     }
     const float o = W == 0.f ? 0.f : O / W;
     if (a.weights || !seg.whole) {
       a.part_o[(static_cast<int64_t>(seg.slot) * kPlainHeads + n) * D + d] = o;
-      if (d == 0) a.part_lse[static_cast<int64_t>(seg.slot) * kPlainHeads + n] = W == 0.f ? -INFINITY : M + log2f(W);
+      if (d == 0) a.part_lse[static_cast<int64_t>(seg.slot) * kPlainHeads + n] = W == 0.f ? -INFINITY : M * a.scale_log2 + log2f(W);
     } else {
       store_any(a.out, a.dtype, (q0 + n) * D + d, o);
     }
