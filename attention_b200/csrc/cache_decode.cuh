@@ -31,105 +31,105 @@ __global__ void __launch_bounds__(kPlainWarps * 32) cache_decode_plain_kernel(co
   Work work(a, pre);
   Segment seg;
   while (work.next<32>(a, pre, seg)) {
-  const int b = seg.b, h = seg.h, head0 = seg.chunk * kPlainHeads, heads = min(kPlainHeads, a.group - head0);
-  const int64_t q0 = static_cast<int64_t>(b) * a.Hq + h * a.group + head0;
-  float q[kPlainHeads][E], acc[kPlainHeads][E], m[kPlainHeads], l[kPlainHeads];
+    const int b = seg.b, h = seg.h, head0 = seg.chunk * kPlainHeads, heads = min(kPlainHeads, a.group - head0);
+    const int64_t q0 = static_cast<int64_t>(b) * a.Hq + h * a.group + head0;
+    float q[kPlainHeads][E], acc[kPlainHeads][E], m[kPlainHeads], l[kPlainHeads];
 #pragma unroll
-  for (int n = 0; n < kPlainHeads; ++n) {
-    m[n] = -INFINITY;
-    l[n] = 0.f;
+    for (int n = 0; n < kPlainHeads; ++n) {
+      m[n] = -INFINITY;
+      l[n] = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
+      for (int e = 0; e < E; ++e) {
+        const int d = lane + 32 * e;
+        q[n][e] = n < heads && d < D ? load_any(a.q, a.dtype, (q0 + n) * D + d) : 0.f;
+        acc[n][e] = 0.f;
+      }
+    }
+    const TilePlan p = tile_plan<32>(a, b);
+    const auto value = [&](const void* base, const __half* scales, int64_t row, int e) -> float {
       const int d = lane + 32 * e;
-      q[n][e] = n < heads && d < D ? load_any(a.q, a.dtype, (q0 + n) * D + d) : 0.f;
-      acc[n][e] = 0.f;
-    }
-  }
-  const TilePlan p = tile_plan<32>(a, b);
-  const auto value = [&](const void* base, const __half* scales, int64_t row, int e) -> float {
-    const int d = lane + 32 * e;
-    if constexpr (sizeof(T) == 1) {
-      const int G = D / kInt4Group;
-      if (e >= G) return 0.f;
-      const uint32_t word = static_cast<const uint16_t*>(base)[row * (G * 8) + (lane >> 2) * G + e];
-      const __half* s = scales + row * 2 * G + e;
-      return fmaf(__half2float(s[0]), static_cast<float>((word >> (4 * (lane & 3))) & 15u), __half2float(s[G]));
-    } else {
-      return d < D ? to_f32<T>(static_cast<const T*>(base)[row * D + d]) : 0.f;
-    }
-  };
-  for (int tile = seg.u0 + warp; tile < seg.u1; tile += kPlainWarps) {
-    const int tok = tile_token<32>(a, p, b, tile, lane);
-    int off = 0;
-    const int page = tok < 0 ? -1 : token_page(a, b, tok, off);
-    const int64_t my_row = page_row(a, b, h, tok, page, off);
-    unsigned live = __ballot_sync(0xffffffffu, my_row >= 0);
-    if (a.scores && tok >= 0 && my_row < 0)
-      for (int n = 0; n < heads; ++n)
-        a.scores[((static_cast<int64_t>(b) * a.Hkv + h) * a.cap + tok) * a.group + head0 + n] = -INFINITY;
-    while (live) {
-      const int i = __ffs(live) - 1;
-      live &= live - 1;
-      const int64_t row = __shfl_sync(0xffffffffu, my_row, i);
-      const int t = __shfl_sync(0xffffffffu, tok, i);
-      float kv[E], s[kPlainHeads];
-#pragma unroll
-      for (int e = 0; e < E; ++e) kv[e] = value(a.k, a.k_scales, row, e);
-#pragma unroll
-      for (int n = 0; n < kPlainHeads; ++n) {
-        s[n] = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) s[n] = fmaf(q[n][e], kv[e], s[n]);
+      if constexpr (sizeof(T) == 1) {
+        const int G = D / kInt4Group;
+        if (e >= G) return 0.f;
+        const uint32_t word = static_cast<const uint16_t*>(base)[row * (G * 8) + (lane >> 2) * G + e];
+        const __half* s = scales + row * 2 * G + e;
+        return fmaf(__half2float(s[0]), static_cast<float>((word >> (4 * (lane & 3))) & 15u), __half2float(s[G]));
+      } else {
+        return d < D ? to_f32<T>(static_cast<const T*>(base)[row * D + d]) : 0.f;
       }
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1)
-#pragma unroll
-        for (int n = 0; n < kPlainHeads; ++n) s[n] += __shfl_xor_sync(0xffffffffu, s[n], off);
-#pragma unroll
-      for (int e = 0; e < E; ++e) kv[e] = value(a.v, a.v_scales, row, e);
-#pragma unroll
-      for (int n = 0; n < kPlainHeads; ++n) {
-        // differences first, then their scale: a scaled score would carry its own rounding
-        const float mn = fmaxf(m[n], s[n]);
-        // a first score of -inf leaves nothing to weigh: the difference would be NaN
-        const float alpha = m[n] == -INFINITY ? 0.f : exp2f((m[n] - mn) * a.scale_log2);
-        const float pr = s[n] == -INFINITY ? 0.f : exp2f((s[n] - mn) * a.scale_log2);
-        l[n] = l[n] * alpha + pr;
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[n][e] = fmaf(acc[n][e], alpha, pr * kv[e]);
-        m[n] = mn;
-      }
-      if (a.scores && lane == 0)
+    };
+    for (int tile = seg.u0 + warp; tile < seg.u1; tile += kPlainWarps) {
+      const int tok = tile_token<32>(a, p, b, tile, lane);
+      int off = 0;
+      const int page = tok < 0 ? -1 : token_page(a, b, tok, off);
+      const int64_t my_row = page_row(a, b, h, tok, page, off);
+      unsigned live = __ballot_sync(0xffffffffu, my_row >= 0);
+      if (a.scores && tok >= 0 && my_row < 0)
         for (int n = 0; n < heads; ++n)
-          a.scores[((static_cast<int64_t>(b) * a.Hkv + h) * a.cap + t) * a.group + head0 + n] = s[n] * a.scale_log2;
-    }
-  }
-  // merge the warps
+          a.scores[((static_cast<int64_t>(b) * a.Hkv + h) * a.cap + tok) * a.group + head0 + n] = -INFINITY;
+      while (live) {
+        const int i = __ffs(live) - 1;
+        live &= live - 1;
+        const int64_t row = __shfl_sync(0xffffffffu, my_row, i);
+        const int t = __shfl_sync(0xffffffffu, tok, i);
+        float kv[E], s[kPlainHeads];
 #pragma unroll
-  for (int n = 0; n < kPlainHeads; ++n) {
-    if (lane == 0) sm[warp][n] = m[n], sl[warp][n] = l[n];
+        for (int e = 0; e < E; ++e) kv[e] = value(a.k, a.k_scales, row, e);
 #pragma unroll
-    for (int e = 0; e < E; ++e) so[warp][n][lane + 32 * e] = acc[n][e];
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < heads * D; i += kPlainWarps * 32) {
-    const int n = i / D, d = i % D;
-    float M = -INFINITY, W = 0.f, O = 0.f;
-    for (int w = 0; w < kPlainWarps; ++w) M = fmaxf(M, sm[w][n]);
-    for (int w = 0; w < kPlainWarps; ++w) {
-      const float f = sm[w][n] == -INFINITY ? 0.f : exp2f((sm[w][n] - M) * a.scale_log2);
-      W = fmaf(sl[w][n], f, W);
-      O = fmaf(so[w][n][d], f, O);
+        for (int n = 0; n < kPlainHeads; ++n) {
+          s[n] = 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) s[n] = fmaf(q[n][e], kv[e], s[n]);
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1)
+#pragma unroll
+          for (int n = 0; n < kPlainHeads; ++n) s[n] += __shfl_xor_sync(0xffffffffu, s[n], off);
+#pragma unroll
+        for (int e = 0; e < E; ++e) kv[e] = value(a.v, a.v_scales, row, e);
+#pragma unroll
+        for (int n = 0; n < kPlainHeads; ++n) {
+          // differences first, then their scale: a scaled score would carry its own rounding
+          const float mn = fmaxf(m[n], s[n]);
+          // a first score of -inf leaves nothing to weigh: the difference would be NaN
+          const float alpha = m[n] == -INFINITY ? 0.f : exp2f((m[n] - mn) * a.scale_log2);
+          const float pr = s[n] == -INFINITY ? 0.f : exp2f((s[n] - mn) * a.scale_log2);
+          l[n] = l[n] * alpha + pr;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[n][e] = fmaf(acc[n][e], alpha, pr * kv[e]);
+          m[n] = mn;
+        }
+        if (a.scores && lane == 0)
+          for (int n = 0; n < heads; ++n)
+            a.scores[((static_cast<int64_t>(b) * a.Hkv + h) * a.cap + t) * a.group + head0 + n] = s[n] * a.scale_log2;
+      }
     }
-    const float o = W == 0.f ? 0.f : O / W;
-    if (a.weights || !seg.whole) {
-      a.part_o[(static_cast<int64_t>(seg.slot) * kPlainHeads + n) * D + d] = o;
-      if (d == 0) a.part_lse[static_cast<int64_t>(seg.slot) * kPlainHeads + n] = W == 0.f ? -INFINITY : M * a.scale_log2 + log2f(W);
-    } else {
-      store_any(a.out, a.dtype, (q0 + n) * D + d, o);
+    // merge the warps
+#pragma unroll
+    for (int n = 0; n < kPlainHeads; ++n) {
+      if (lane == 0) sm[warp][n] = m[n], sl[warp][n] = l[n];
+#pragma unroll
+      for (int e = 0; e < E; ++e) so[warp][n][lane + 32 * e] = acc[n][e];
     }
-  }
-  __syncthreads();  // the next segment reuses the buffers
+    __syncthreads();
+    for (int i = threadIdx.x; i < heads * D; i += kPlainWarps * 32) {
+      const int n = i / D, d = i % D;
+      float M = -INFINITY, W = 0.f, O = 0.f;
+      for (int w = 0; w < kPlainWarps; ++w) M = fmaxf(M, sm[w][n]);
+      for (int w = 0; w < kPlainWarps; ++w) {
+        const float f = sm[w][n] == -INFINITY ? 0.f : exp2f((sm[w][n] - M) * a.scale_log2);
+        W = fmaf(sl[w][n], f, W);
+        O = fmaf(so[w][n][d], f, O);
+      }
+      const float o = W == 0.f ? 0.f : O / W;
+      if (a.weights || !seg.whole) {
+        a.part_o[(static_cast<int64_t>(seg.slot) * kPlainHeads + n) * D + d] = o;
+        if (d == 0) a.part_lse[static_cast<int64_t>(seg.slot) * kPlainHeads + n] = W == 0.f ? -INFINITY : M * a.scale_log2 + log2f(W);
+      } else {
+        store_any(a.out, a.dtype, (q0 + n) * D + d, o);
+      }
+    }
+    __syncthreads();  // the next segment reuses the buffers
   }
 }
 

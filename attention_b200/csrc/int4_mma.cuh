@@ -205,488 +205,488 @@ __global__ void __launch_bounds__(Int4Cfg<G, NT>::kWarps * 32, Int4Cfg<G, NT>::k
   Segment seg;
 #pragma unroll 1
   while (work.next<S::kTok>(a, pre, seg)) {
-  const int b = seg.b, h = seg.h, head0 = seg.chunk * HN, heads = min(HN, a.group - head0);
-  const int64_t q0 = static_cast<int64_t>(b) * a.Hq + h * a.group + head0;
-  const TilePlan plan = tile_plan<S::kTok>(a, b);
+    const int b = seg.b, h = seg.h, head0 = seg.chunk * HN, heads = min(HN, a.group - head0);
+    const int64_t q0 = static_cast<int64_t>(b) * a.Hq + h * a.group + head0;
+    const TilePlan plan = tile_plan<S::kTok>(a, b);
 
-  int next_tile, end_tile;  // this warp's tiles, one stretch
-  split_range(seg.u1 - seg.u0, warp, W, next_tile, end_tile);
-  next_tile += seg.u0, end_tile += seg.u0;
-  const int first_tile = next_tile, n_tiles = end_tile - next_tile;
+    int next_tile, end_tile;  // this warp's tiles, one stretch
+    split_range(seg.u1 - seg.u0, warp, W, next_tile, end_tile);
+    next_tile += seg.u0, end_tile += seg.u0;
+    const int first_tile = next_tile, n_tiles = end_tile - next_tile;
 
-  // ---- rows of the next tiles.  A tile's page is fetched one tile before its loads are issued.
-  // A full tile inside one page takes one look-up, good for the `run` full tiles that are left in
-  // the page, from row `flat` on; other tiles have a token, a page and a row a lane.
-  int token = -1, page = -1, page_off = 0, run = 0, flat = 0;
-  bool one_page = false;
-  const auto fetch = [&]() {
-    const int first = tile_token<S::kTok>(a, plan, b, next_tile, 0), last = tile_token<S::kTok>(a, plan, b, next_tile, S::kTok - 1);
-    one_page = false;
-    if (first >= 0 && last >= 0) {
-      page = token_page(a, b, first, page_off);
-      token = first;
-      one_page = page_off + S::kTok <= a.addr.page_size;
-    }
-    if (!one_page) {
-      token = tile_token<S::kTok>(a, plan, b, next_tile, lane);
-      page = token < 0 ? -1 : token_page(a, b, token, page_off);
-    }
-  };
-  if (next_tile < end_tile) fetch();
-  const unsigned char* k_lane = static_cast<const unsigned char*>(a.k) + lane * 16;
-  const unsigned char* v_lane = static_cast<const unsigned char*>(a.v) + lane * 16;
-  const unsigned char* kz_lane = reinterpret_cast<const unsigned char*>(a.k_scales) + lane * S::kScaleChunk;
-  const unsigned char* vz_lane = reinterpret_cast<const unsigned char*>(a.v_scales) + lane * S::kScaleChunk;
-  const int put = S::at(lane / G, lane % G * 16);
-  const auto issue = [&](int stage) {
-    if (next_tile < end_tile) {
-      const uint32_t base = smem_u32(ring + stage * S::kStage);
-      constexpr int per = S::kScaleRow / S::kScaleChunk;
-      int row = -1;
-      if (run == 0) {
-        row = static_cast<int>(page_row(a, b, h, token, page, page_off));
-        if (one_page && row >= 0) {
-          flat = row;
-          run = min(a.addr.page_size - page_off, plan.ctx - token) / S::kTok;
-        }
+    // ---- rows of the next tiles.  A tile's page is fetched one tile before its loads are issued.
+    // A full tile inside one page takes one look-up, good for the `run` full tiles that are left in
+    // the page, from row `flat` on; other tiles have a token, a page and a row a lane.
+    int token = -1, page = -1, page_off = 0, run = 0, flat = 0;
+    bool one_page = false;
+    const auto fetch = [&]() {
+      const int first = tile_token<S::kTok>(a, plan, b, next_tile, 0), last = tile_token<S::kTok>(a, plan, b, next_tile, S::kTok - 1);
+      one_page = false;
+      if (first >= 0 && last >= 0) {
+        page = token_page(a, b, first, page_off);
+        token = first;
+        one_page = page_off + S::kTok <= a.addr.page_size;
       }
-      if (run > 0) {
-        // 32 rows on end: one address an array
-        if (lane == 0) s_live[warp][stage] = 0xffffffffu;
-        const unsigned char* kp = k_lane + static_cast<int64_t>(flat) * S::kRow;
-        const unsigned char* vp = v_lane + static_cast<int64_t>(flat) * S::kRow;
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-          const int c = i * 32 + lane;
-          // 8 rows on, the permutation is the same
-          const uint32_t dst = base + (32 / G % 8 == 0 && 32 % G == 0 ? put + i * 512 : S::at(c / G, (c % G) * 16));
-          cp_async<16>(dst, kp + i * 512, 16);
-          cp_async<16>(dst + S::kCodes, vp + i * 512, 16);
-        }
-        const unsigned char* kz = kz_lane + static_cast<int64_t>(flat) * S::kScaleRow;
-        const unsigned char* vz = vz_lane + static_cast<int64_t>(flat) * S::kScaleRow;
-#pragma unroll
-        for (int i = 0; i < per; ++i) {
-          const uint32_t dst = base + 2 * S::kCodes + (i * 32 + lane) * S::kScaleChunk;
-          cp_async<S::kScaleChunk>(dst, kz + i * 32 * S::kScaleChunk, S::kScaleChunk);
-          cp_async<S::kScaleChunk>(dst + S::kScales, vz + i * 32 * S::kScaleChunk, S::kScaleChunk);
-        }
-        flat += S::kTok;
-        --run;
-      } else {
-        const unsigned live = __ballot_sync(0xffffffffu, row >= 0);
-        if (lane == 0) s_live[warp][stage] = live;
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-          const int c = i * 32 + lane, tok = c / G, off = (c % G) * 16;
-          const int r = __shfl_sync(0xffffffffu, row, tok);
-          const int64_t src = static_cast<int64_t>(max(r, 0)) * S::kRow + off;
-          const int n = r >= 0 ? 16 : 0;
-          cp_async<16>(base + S::at(tok, off), static_cast<const unsigned char*>(a.k) + src, n);
-          cp_async<16>(base + S::kCodes + S::at(tok, off), static_cast<const unsigned char*>(a.v) + src, n);
-        }
-#pragma unroll
-        for (int i = 0; i < per; ++i) {
-          const int c = i * 32 + lane, tok = c / per, off = (c % per) * S::kScaleChunk;
-          const int r = __shfl_sync(0xffffffffu, row, tok);
-          const int64_t src = static_cast<int64_t>(max(r, 0)) * S::kScaleRow + off;
-          const int n = r >= 0 ? S::kScaleChunk : 0;
-          const uint32_t dst = base + 2 * S::kCodes + tok * S::kScaleRow + off;
-          cp_async<S::kScaleChunk>(dst, reinterpret_cast<const unsigned char*>(a.k_scales) + src, n);
-          cp_async<S::kScaleChunk>(dst + S::kScales, reinterpret_cast<const unsigned char*>(a.v_scales) + src, n);
-        }
+      if (!one_page) {
+        token = tile_token<S::kTok>(a, plan, b, next_tile, lane);
+        page = token < 0 ? -1 : token_page(a, b, token, page_off);
       }
-      if (++next_tile < end_tile && run == 0) fetch();
-    }
-    cp_async_commit();
-  };
-  issue(0);
-
-  // ---- the queries as B fragments, a group of 32 values (of 8 heads) a warp.  A row is scaled
-  // by a power of two to a largest value in [2^9, 2^10): fp16 then holds 16-bit queries exactly,
-  // and group sums stay in range.
-  float x[8], big = 0.f;
-  if (warp < NT * G) {
-    const int head = warp / G * 8 + g;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    if (head < heads) load8_any(a.q, a.dtype, (q0 + head) * D + 32 * (warp % G) + 8 * t, a.q_vec, x);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(x[i]));
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-    s_big[warp][g] = big;
-  }
-  __syncthreads();
-  if (warp < NT * G) {
-    const int n = warp / G;
-#pragma unroll
-    for (int j = 0; j < G; ++j) big = fmaxf(big, s_big[n * G + j][g]);
-    int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;  // floor(log2) of a normal number
-    e = big == 0.f || e == 128 ? 9 : min(max(e, -110), 120);
-    const float up = __uint_as_float(static_cast<uint32_t>(127 - e + 9) << 23);
-    s_unit[n * 8 + g] = __uint_as_float(static_cast<uint32_t>(127 + e - 9) << 23) * a.scale_log2;
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum += x[i] *= up;
-    uint32_t hi[4], lo[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float f = !kCentreK && i & 1 ? 0.0625f : 1.f;
-      hi[i] = pack_h2(x[i] * f, x[i + 4] * f);
-      lo[i] = pack_h2(x[i] * f - half_lo(hi[i]), x[i + 4] * f - half_hi(hi[i]));
-    }
-    *reinterpret_cast<uint4*>(s_q[0][warp][lane]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    if constexpr (PREC == 2) *reinterpret_cast<uint4*>(s_q[PREC == 2][warp][lane]) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    s_sum[warp][g] = sum;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int s = 1; s < ST - 1; ++s) issue(s);
-  uint32_t qb[NT][G][2][2], ql[NT][G][2][2], qz[NT][2];
-  float q_unit[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int j = 0; j < G; ++j) {
-      *reinterpret_cast<uint4*>(&qb[n][j][0][0]) = *reinterpret_cast<const uint4*>(s_q[0][n * G + j][lane]);
-      if constexpr (PREC == 2)
-        *reinterpret_cast<uint4*>(&ql[n][j][0][0]) = *reinterpret_cast<const uint4*>(s_q[PREC == 2][n * G + j][lane]);
-    }
-    q_unit[n][0] = s_unit[n * 8 + 2 * t];
-    q_unit[n][1] = s_unit[n * 8 + 2 * t + 1];
-    // sums of groups 2t and 2t + 1
-    const float z0 = 2 * t < G ? s_sum[n * G + 2 * t][g] : 0.f, z1 = 2 * t + 1 < G ? s_sum[n * G + 2 * t + 1][g] : 0.f;
-    qz[n][0] = pack_h2(z0, z1);
-    qz[n][1] = pack_h2(z0 - half_lo(qz[n][0]), z1 - half_hi(qz[n][0]));
-  }
-  // a lane's places in a stage; 8 rows on, the permutation is the same
-  const int k_at = S::at(g, 4 * G * t), k_at2 = G == 8 ? S::at(g, 4 * G * t + 16) : 0;
-  const int v_at = S::at(2 * t, 2 * G * g), v_at1 = S::at(2 * t + 1, 2 * G * g);
-
-  // m: about the largest score so far, in the scaled query's units; base2: what an exponent starts from,
-  // log2(unit) - m * q_unit
-  float o[NT][G][2][4], zo[NT][4], m[NT][2], limit[NT][2], base2[NT][2], l[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int j = 0; j < G; ++j)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[n][j][u][e] = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) zo[n][e] = 0.f;
-    m[n][0] = m[n][1] = -INFINITY;
-    limit[n][0] = limit[n][1] = -INFINITY;
-    base2[n][0] = base2[n][1] = kUnit2;
-    l[n][0] = l[n][1] = 0.f;
-  }
-  // Probabilities and all sums of them are held times unit = 2^(15 - kSlack) / top, top a power
-  // of two no V scale so far exceeds (1 at least): fp16 then holds p and p s, and the lower
-  // halves of those, over the widest range.
-  uint32_t top = 0x3c00u;
-  float unit2 = kUnit2;
-  // z + 8 s is held as it is, or, once scales above kWide = 4096 turned up (it might pass fp16's
-  // range), in sixteenths
-  constexpr uint32_t kWide = 0x6c00u;
-  float z_unit = 1.f;
-
-  int stage = 0;
-#pragma unroll 1
-  for (int done = 0; done < n_tiles; ++done) {
-    cp_async_wait<ST - 2>();
-    __syncwarp();
-    issue(stage == 0 ? ST - 1 : stage - 1);  // the stage that the previous tile left
-    const unsigned char* ks = ring + stage * S::kStage;
-    const unsigned char* vs = ks + S::kCodes;
-    const unsigned char* ksc = ks + 2 * S::kCodes;
-    const unsigned char* vsc = ksc + S::kScales;
-    const unsigned live = s_live[warp][stage];
-    float sc[2][NT][4], mn[NT][2];
-    float zk_unit = 1.f;  // as z_unit, for this tile of K
-    if constexpr (kCentreK) {
-      uint32_t ktop[(G + 1) / 2], most = 0;
-      lds_words<2 * G>(ksc + lane * S::kScaleRow, ktop);
-#pragma unroll
-      for (int i = 0; i < (G + 1) / 2; ++i) most = __vmaxu2(most, ktop[i]);
-      if (__any_sync(0xffffffffu, max(most & 0xffffu, most >> 16) > kWide)) zk_unit = 0.0625f;
-    }
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      const int r0 = hh * 16 + g, r1 = r0 + 8;
-      uint32_t w0[G], w1[G], s0[(G + 1) / 2], s1[(G + 1) / 2];
-      const unsigned char* kr = ks + hh * 16 * S::kRow;
-      if constexpr (G == 8) {
-        lds_words<16>(kr + k_at, w0);
-        lds_words<16>(kr + k_at2, w0 + 4);
-        lds_words<16>(kr + 8 * S::kRow + k_at, w1);
-        lds_words<16>(kr + 8 * S::kRow + k_at2, w1 + 4);
-      } else {
-        lds_words<4 * G>(kr + k_at, w0);
-        lds_words<4 * G>(kr + 8 * S::kRow + k_at, w1);
-      }
-      lds_words<2 * G>(ksc + r0 * S::kScaleRow, s0);
-      lds_words<2 * G>(ksc + r1 * S::kScaleRow, s1);
-      // zeros of groups 2t and 2t + 1; past G any of the row's will do: the query sums are 0 there
-      const auto pair_at = [&](int r, int first) -> uint32_t {
-        const unsigned char* p = ksc + r * S::kScaleRow + 2 * first;
-        if constexpr (G % 2 == 0) return reinterpret_cast<const uint32_t*>(p)[t % (G / 2)];
-        const unsigned short* x = reinterpret_cast<const unsigned short*>(p);
-        return __byte_perm(x[2 * t % G], x[(2 * t + 1) % G], 0x5410);
-      };
-      uint32_t z0 = pair_at(r0, G), z1 = pair_at(r1, G), zl0 = 0, zl1 = 0;
-      if constexpr (kCentreK) {
-        centre_zero(z0, zl0, pair_at(r0, 0), zk_unit);
-        centre_zero(z1, zl1, pair_at(r1, 0), zk_unit);
-      }
-      float acc[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-      const auto group = [&](auto jc) {
-        constexpr int j = decltype(jc)::value;
-        uint32_t x0[4], x1[4];
-        nibbles<kCentreK>(pair16<j, G + j>(w0, w0), x0);
-        nibbles<kCentreK>(pair16<j, G + j>(w1, w1), x1);
-        const float f0 = j & 1 ? half_hi(s0[j / 2]) : half_lo(s0[j / 2]);
-        const float f1 = j & 1 ? half_hi(s1[j / 2]) : half_lo(s1[j / 2]);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float c[4];
-          mma_f16_zero(c, x0[0], x1[0], x0[1], x1[1], qb[n][j][0][0], qb[n][j][0][1]);
-          mma_f16(c, x0[2], x1[2], x0[3], x1[3], qb[n][j][1][0], qb[n][j][1][1]);
-          if constexpr (PREC == 2) {
-            mma_f16(c, x0[0], x1[0], x0[1], x1[1], ql[n][j][0][0], ql[n][j][0][1]);
-            mma_f16(c, x0[2], x1[2], x0[3], x1[3], ql[n][j][1][0], ql[n][j][1][1]);
+    };
+    if (next_tile < end_tile) fetch();
+    const unsigned char* k_lane = static_cast<const unsigned char*>(a.k) + lane * 16;
+    const unsigned char* v_lane = static_cast<const unsigned char*>(a.v) + lane * 16;
+    const unsigned char* kz_lane = reinterpret_cast<const unsigned char*>(a.k_scales) + lane * S::kScaleChunk;
+    const unsigned char* vz_lane = reinterpret_cast<const unsigned char*>(a.v_scales) + lane * S::kScaleChunk;
+    const int put = S::at(lane / G, lane % G * 16);
+    const auto issue = [&](int stage) {
+      if (next_tile < end_tile) {
+        const uint32_t base = smem_u32(ring + stage * S::kStage);
+        constexpr int per = S::kScaleRow / S::kScaleChunk;
+        int row = -1;
+        if (run == 0) {
+          row = static_cast<int>(page_row(a, b, h, token, page, page_off));
+          if (one_page && row >= 0) {
+            flat = row;
+            run = min(a.addr.page_size - page_off, plan.ctx - token) / S::kTok;
           }
-          acc[n][0] = fmaf(f0, c[0], acc[n][0]);
-          acc[n][1] = fmaf(f0, c[1], acc[n][1]);
-          acc[n][2] = fmaf(f1, c[2], acc[n][2]);
-          acc[n][3] = fmaf(f1, c[3], acc[n][3]);
         }
-      };
-      for_each_index(group, std::make_integer_sequence<int, G>{});
+        if (run > 0) {
+          // 32 rows on end: one address an array
+          if (lane == 0) s_live[warp][stage] = 0xffffffffu;
+          const unsigned char* kp = k_lane + static_cast<int64_t>(flat) * S::kRow;
+          const unsigned char* vp = v_lane + static_cast<int64_t>(flat) * S::kRow;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float c[4];
-        mma_f16_zero(c, z0, z1, z0, z1, qz[n][0], qz[n][1]);
-        if constexpr (kCentreK) mma_f16(c, zl0, zl1, zl0, zl1, qz[n][0], qz[n][1]);
+          for (int i = 0; i < G; ++i) {
+            const int c = i * 32 + lane;
+            // 8 rows on, the permutation is the same
+            const uint32_t dst = base + (32 / G % 8 == 0 && 32 % G == 0 ? put + i * 512 : S::at(c / G, (c % G) * 16));
+            cp_async<16>(dst, kp + i * 512, 16);
+            cp_async<16>(dst + S::kCodes, vp + i * 512, 16);
+          }
+          const unsigned char* kz = kz_lane + static_cast<int64_t>(flat) * S::kScaleRow;
+          const unsigned char* vz = vz_lane + static_cast<int64_t>(flat) * S::kScaleRow;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[hh][n][e] = kCentreK ? fmaf(c[e], 1.f / zk_unit, acc[n][e]) : fmaf(acc[n][e], kUnitK, c[e]);
+          for (int i = 0; i < per; ++i) {
+            const uint32_t dst = base + 2 * S::kCodes + (i * 32 + lane) * S::kScaleChunk;
+            cp_async<S::kScaleChunk>(dst, kz + i * 32 * S::kScaleChunk, S::kScaleChunk);
+            cp_async<S::kScaleChunk>(dst + S::kScales, vz + i * 32 * S::kScaleChunk, S::kScaleChunk);
+          }
+          flat += S::kTok;
+          --run;
+        } else {
+          const unsigned live = __ballot_sync(0xffffffffu, row >= 0);
+          if (lane == 0) s_live[warp][stage] = live;
+#pragma unroll
+          for (int i = 0; i < G; ++i) {
+            const int c = i * 32 + lane, tok = c / G, off = (c % G) * 16;
+            const int r = __shfl_sync(0xffffffffu, row, tok);
+            const int64_t src = static_cast<int64_t>(max(r, 0)) * S::kRow + off;
+            const int n = r >= 0 ? 16 : 0;
+            cp_async<16>(base + S::at(tok, off), static_cast<const unsigned char*>(a.k) + src, n);
+            cp_async<16>(base + S::kCodes + S::at(tok, off), static_cast<const unsigned char*>(a.v) + src, n);
+          }
+#pragma unroll
+          for (int i = 0; i < per; ++i) {
+            const int c = i * 32 + lane, tok = c / per, off = (c % per) * S::kScaleChunk;
+            const int r = __shfl_sync(0xffffffffu, row, tok);
+            const int64_t src = static_cast<int64_t>(max(r, 0)) * S::kScaleRow + off;
+            const int n = r >= 0 ? S::kScaleChunk : 0;
+            const uint32_t dst = base + 2 * S::kCodes + tok * S::kScaleRow + off;
+            cp_async<S::kScaleChunk>(dst, reinterpret_cast<const unsigned char*>(a.k_scales) + src, n);
+            cp_async<S::kScaleChunk>(dst + S::kScales, reinterpret_cast<const unsigned char*>(a.v_scales) + src, n);
+          }
+        }
+        if (++next_tile < end_tile && run == 0) fetch();
       }
-    }
-    if (live != 0xffffffffu) {
+      cp_async_commit();
+    };
+    issue(0);
+
+    // ---- the queries as B fragments, a group of 32 values (of 8 heads) a warp.  A row is scaled
+    // by a power of two to a largest value in [2^9, 2^10): fp16 then holds 16-bit queries exactly,
+    // and group sums stay in range.
+    float x[8], big = 0.f;
+    if (warp < NT * G) {
+      const int head = warp / G * 8 + g;
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh)
+      for (int i = 0; i < 8; ++i) x[i] = 0.f;
+      if (head < heads) load8_any(a.q, a.dtype, (q0 + head) * D + 32 * (warp % G) + 8 * t, a.q_vec, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(x[i]));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      s_big[warp][g] = big;
+    }
+    __syncthreads();
+    if (warp < NT * G) {
+      const int n = warp / G;
+#pragma unroll
+      for (int j = 0; j < G; ++j) big = fmaxf(big, s_big[n * G + j][g]);
+      int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;  // floor(log2) of a normal number
+      e = big == 0.f || e == 128 ? 9 : min(max(e, -110), 120);
+      const float up = __uint_as_float(static_cast<uint32_t>(127 - e + 9) << 23);
+      s_unit[n * 8 + g] = __uint_as_float(static_cast<uint32_t>(127 + e - 9) << 23) * a.scale_log2;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += x[i] *= up;
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f = !kCentreK && i & 1 ? 0.0625f : 1.f;
+        hi[i] = pack_h2(x[i] * f, x[i + 4] * f);
+        lo[i] = pack_h2(x[i] * f - half_lo(hi[i]), x[i + 4] * f - half_hi(hi[i]));
+      }
+      *reinterpret_cast<uint4*>(s_q[0][warp][lane]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      if constexpr (PREC == 2) *reinterpret_cast<uint4*>(s_q[PREC == 2][warp][lane]) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      s_sum[warp][g] = sum;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 1; s < ST - 1; ++s) issue(s);
+    uint32_t qb[NT][G][2][2], ql[NT][G][2][2], qz[NT][2];
+    float q_unit[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        *reinterpret_cast<uint4*>(&qb[n][j][0][0]) = *reinterpret_cast<const uint4*>(s_q[0][n * G + j][lane]);
+        if constexpr (PREC == 2)
+          *reinterpret_cast<uint4*>(&ql[n][j][0][0]) = *reinterpret_cast<const uint4*>(s_q[PREC == 2][n * G + j][lane]);
+      }
+      q_unit[n][0] = s_unit[n * 8 + 2 * t];
+      q_unit[n][1] = s_unit[n * 8 + 2 * t + 1];
+      // sums of groups 2t and 2t + 1
+      const float z0 = 2 * t < G ? s_sum[n * G + 2 * t][g] : 0.f, z1 = 2 * t + 1 < G ? s_sum[n * G + 2 * t + 1][g] : 0.f;
+      qz[n][0] = pack_h2(z0, z1);
+      qz[n][1] = pack_h2(z0 - half_lo(qz[n][0]), z1 - half_hi(qz[n][0]));
+    }
+    // a lane's places in a stage; 8 rows on, the permutation is the same
+    const int k_at = S::at(g, 4 * G * t), k_at2 = G == 8 ? S::at(g, 4 * G * t + 16) : 0;
+    const int v_at = S::at(2 * t, 2 * G * g), v_at1 = S::at(2 * t + 1, 2 * G * g);
+
+    // m: about the largest score so far, in the scaled query's units; base2: what an exponent starts from,
+    // log2(unit) - m * q_unit
+    float o[NT][G][2][4], zo[NT][4], m[NT][2], limit[NT][2], base2[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int j = 0; j < G; ++j)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][j][u][e] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) zo[n][e] = 0.f;
+      m[n][0] = m[n][1] = -INFINITY;
+      limit[n][0] = limit[n][1] = -INFINITY;
+      base2[n][0] = base2[n][1] = kUnit2;
+      l[n][0] = l[n][1] = 0.f;
+    }
+    // Probabilities and all sums of them are held times unit = 2^(15 - kSlack) / top, top a power
+    // of two no V scale so far exceeds (1 at least): fp16 then holds p and p s, and the lower
+    // halves of those, over the widest range.
+    uint32_t top = 0x3c00u;
+    float unit2 = kUnit2;
+    // z + 8 s is held as it is, or, once scales above kWide = 4096 turned up (it might pass fp16's
+    // range), in sixteenths
+    constexpr uint32_t kWide = 0x6c00u;
+    float z_unit = 1.f;
+
+    int stage = 0;
+#pragma unroll 1
+    for (int done = 0; done < n_tiles; ++done) {
+      cp_async_wait<ST - 2>();
+      __syncwarp();
+      issue(stage == 0 ? ST - 1 : stage - 1);  // the stage that the previous tile left
+      const unsigned char* ks = ring + stage * S::kStage;
+      const unsigned char* vs = ks + S::kCodes;
+      const unsigned char* ksc = ks + 2 * S::kCodes;
+      const unsigned char* vsc = ksc + S::kScales;
+      const unsigned live = s_live[warp][stage];
+      float sc[2][NT][4], mn[NT][2];
+      float zk_unit = 1.f;  // as z_unit, for this tile of K
+      if constexpr (kCentreK) {
+        uint32_t ktop[(G + 1) / 2], most = 0;
+        lds_words<2 * G>(ksc + lane * S::kScaleRow, ktop);
+#pragma unroll
+        for (int i = 0; i < (G + 1) / 2; ++i) most = __vmaxu2(most, ktop[i]);
+        if (__any_sync(0xffffffffu, max(most & 0xffffu, most >> 16) > kWide)) zk_unit = 0.0625f;
+      }
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const int r0 = hh * 16 + g, r1 = r0 + 8;
+        uint32_t w0[G], w1[G], s0[(G + 1) / 2], s1[(G + 1) / 2];
+        const unsigned char* kr = ks + hh * 16 * S::kRow;
+        if constexpr (G == 8) {
+          lds_words<16>(kr + k_at, w0);
+          lds_words<16>(kr + k_at2, w0 + 4);
+          lds_words<16>(kr + 8 * S::kRow + k_at, w1);
+          lds_words<16>(kr + 8 * S::kRow + k_at2, w1 + 4);
+        } else {
+          lds_words<4 * G>(kr + k_at, w0);
+          lds_words<4 * G>(kr + 8 * S::kRow + k_at, w1);
+        }
+        lds_words<2 * G>(ksc + r0 * S::kScaleRow, s0);
+        lds_words<2 * G>(ksc + r1 * S::kScaleRow, s1);
+        // zeros of groups 2t and 2t + 1; past G any of the row's will do: the query sums are 0 there
+        const auto pair_at = [&](int r, int first) -> uint32_t {
+          const unsigned char* p = ksc + r * S::kScaleRow + 2 * first;
+          if constexpr (G % 2 == 0) return reinterpret_cast<const uint32_t*>(p)[t % (G / 2)];
+          const unsigned short* x = reinterpret_cast<const unsigned short*>(p);
+          return __byte_perm(x[2 * t % G], x[(2 * t + 1) % G], 0x5410);
+        };
+        uint32_t z0 = pair_at(r0, G), z1 = pair_at(r1, G), zl0 = 0, zl1 = 0;
+        if constexpr (kCentreK) {
+          centre_zero(z0, zl0, pair_at(r0, 0), zk_unit);
+          centre_zero(z1, zl1, pair_at(r1, 0), zk_unit);
+        }
+        float acc[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!(live >> (hh * 16 + g + (e < 2 ? 0 : 8)) & 1)) sc[hh][n][e] = -INFINITY;
-    }
-    if (a.scores) {
-      // [token][head of the group]; a lane's two heads lie on end
-      const int64_t at = (static_cast<int64_t>(b) * a.Hkv + h) * a.cap;
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          const int tok = plan.seg + (first_tile + done) * S::kTok + hh * 16 + g + 4 * e;
-          if (tok < plan.lo || tok >= plan.ctx) continue;
+          for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+        const auto group = [&](auto jc) {
+          constexpr int j = decltype(jc)::value;
+          uint32_t x0[4], x1[4];
+          nibbles<kCentreK>(pair16<j, G + j>(w0, w0), x0);
+          nibbles<kCentreK>(pair16<j, G + j>(w1, w1), x1);
+          const float f0 = j & 1 ? half_hi(s0[j / 2]) : half_lo(s0[j / 2]);
+          const float f1 = j & 1 ? half_hi(s1[j / 2]) : half_lo(s1[j / 2]);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const int head = n * 8 + 2 * t;
-            float* p = a.scores + (at + tok) * a.group + head0 + head;
-            const float x = sc[hh][n][e] * q_unit[n][0], y = sc[hh][n][e + 1] * q_unit[n][1];
-            if (head + 1 < heads && a.group % 2 == 0) {
-              *reinterpret_cast<float2*>(p) = make_float2(x, y);
-            } else if (head < heads) {
-              p[0] = x;
-              if (head + 1 < heads) p[1] = y;
+            float c[4];
+            mma_f16_zero(c, x0[0], x1[0], x0[1], x1[1], qb[n][j][0][0], qb[n][j][0][1]);
+            mma_f16(c, x0[2], x1[2], x0[3], x1[3], qb[n][j][1][0], qb[n][j][1][1]);
+            if constexpr (PREC == 2) {
+              mma_f16(c, x0[0], x1[0], x0[1], x1[1], ql[n][j][0][0], ql[n][j][0][1]);
+              mma_f16(c, x0[2], x1[2], x0[3], x1[3], ql[n][j][1][0], ql[n][j][1][1]);
             }
+            acc[n][0] = fmaf(f0, c[0], acc[n][0]);
+            acc[n][1] = fmaf(f0, c[1], acc[n][1]);
+            acc[n][2] = fmaf(f1, c[2], acc[n][2]);
+            acc[n][3] = fmaf(f1, c[3], acc[n][3]);
           }
+        };
+        for_each_index(group, std::make_integer_sequence<int, G>{});
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float c[4];
+          mma_f16_zero(c, z0, z1, z0, z1, qz[n][0], qz[n][1]);
+          if constexpr (kCentreK) mma_f16(c, zl0, zl1, zl0, zl1, qz[n][0], qz[n][1]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[hh][n][e] = kCentreK ? fmaf(c[e], 1.f / zk_unit, acc[n][e]) : fmaf(acc[n][e], kUnitK, c[e]);
         }
-    }
-    // ---- running maximum and sum.  The maximum is only moved once a score passes it by
-    // 2^kSlack: until then probabilities reach 2^kSlack instead of 1, for which unit leaves room.
-    bool up = false;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        mn[n][c] = fmaxf(fmaxf(sc[0][n][c], sc[0][n][2 + c]), fmaxf(sc[1][n][c], sc[1][n][2 + c]));
-        up |= mn[n][c] > limit[n][c];
       }
-    // largest V scale of the tile: this lane's token (NaN and negative ones count as fp16's largest)
-    uint32_t vtop[(G + 1) / 2], most = 0;
-    lds_words<2 * G>(vsc + lane * S::kScaleRow, vtop);
+      if (live != 0xffffffffu) {
 #pragma unroll
-    for (int i = 0; i < (G + 1) / 2; ++i) most = __vmaxu2(most, vtop[i]);
-    most = max(most & 0xffffu, most >> 16);
-    if (__any_sync(0xffffffffu, up || most > top)) {
-      float shrink = 1.f;
-      const uint32_t all = min(__reduce_max_sync(0xffffffffu, most), 0x7bffu);
-      if (all > top) {
-        const uint32_t to = (all + 0x3ffu) & 0x7c00u;  // the next power of two
-        shrink = __uint_as_float((127u - ((to - top) >> 10)) << 23);
-        unit2 -= static_cast<float>((to - top) >> 10);
-        if (to > kWide && top <= kWide) {
-          z_unit = 0.0625f;
+        for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) zo[n][e] *= z_unit;
-        }
-        top = to;
+            for (int e = 0; e < 4; ++e)
+              if (!(live >> (hh * 16 + g + (e < 2 ? 0 : 8)) & 1)) sc[hh][n][e] = -INFINITY;
       }
+      if (a.scores) {
+        // [token][head of the group]; a lane's two heads lie on end
+        const int64_t at = (static_cast<int64_t>(b) * a.Hkv + h) * a.cap;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float f[2];
+        for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float x = mn[n][c];
+          for (int e = 0; e < 4; e += 2) {
+            const int tok = plan.seg + (first_tile + done) * S::kTok + hh * 16 + g + 4 * e;
+            if (tok < plan.lo || tok >= plan.ctx) continue;
 #pragma unroll
-          for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-          x = fmaxf(m[n][c], x);
-          // nothing seen yet: 0, not exp2(-inf + inf)
-          f[c] = m[n][c] == -INFINITY ? 0.f : fast_exp2((m[n][c] - x) * q_unit[n][c]) * shrink;
-          l[n][c] *= f[c];
-          m[n][c] = x;
-          limit[n][c] = x + kSlack / q_unit[n][c];
-          base2[n][c] = x == -INFINITY ? unit2 : fmaf(-x, q_unit[n][c], unit2);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) zo[n][e] *= f[e & 1];
-#pragma unroll
-        for (int j = 0; j < G; ++j)
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][j][u][e] *= f[e & 1];
+            for (int n = 0; n < NT; ++n) {
+              const int head = n * 8 + 2 * t;
+              float* p = a.scores + (at + tok) * a.group + head0 + head;
+              const float x = sc[hh][n][e] * q_unit[n][0], y = sc[hh][n][e + 1] * q_unit[n][1];
+              if (head + 1 < heads && a.group % 2 == 0) {
+                *reinterpret_cast<float2*>(p) = make_float2(x, y);
+              } else if (head < heads) {
+                p[0] = x;
+                if (head + 1 < heads) p[1] = y;
+              }
+            }
+          }
       }
-    }
-    // ---- P V
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      float p[NT][4];
+      // ---- running maximum and sum.  The maximum is only moved once a score passes it by
+      // 2^kSlack: until then probabilities reach 2^kSlack instead of 1, for which unit leaves room.
+      bool up = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          p[n][e] = fast_exp2(fmaf(sc[hh][n][e], q_unit[n][e & 1], base2[n][e & 1]));
-          l[n][e & 1] += p[n][e];
+        for (int c = 0; c < 2; ++c) {
+          mn[n][c] = fmaxf(fmaxf(sc[0][n][c], sc[0][n][2 + c]), fmaxf(sc[1][n][c], sc[1][n][2 + c]));
+          up |= mn[n][c] > limit[n][c];
         }
-      const int rt = hh * 16 + 2 * t;  // this lane's tokens in the product: rt, rt+1, rt+8, rt+9
-      uint32_t v0[(G + 1) / 2], v1[(G + 1) / 2], v2[(G + 1) / 2], v3[(G + 1) / 2];
-      const unsigned char* vr = vs + hh * 16 * S::kRow;
-      lds_words<2 * G>(vr + v_at, v0);
-      lds_words<2 * G>(vr + v_at1, v1);
-      lds_words<2 * G>(vr + 8 * S::kRow + v_at, v2);
-      lds_words<2 * G>(vr + 8 * S::kRow + v_at1, v3);
-      uint32_t b0[NT], b1[NT], bl0[NT], bl1[NT];
+      // largest V scale of the tile: this lane's token (NaN and negative ones count as fp16's largest)
+      uint32_t vtop[(G + 1) / 2], most = 0;
+      lds_words<2 * G>(vsc + lane * S::kScaleRow, vtop);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const uint32_t h0 = pack_h2(p[n][0], p[n][1]), h1 = pack_h2(p[n][2], p[n][3]);
-        b0[n] = movmatrix_trans(h0);
-        b1[n] = movmatrix_trans(h1);
-        if constexpr (PREC > 0) {
-          bl0[n] = movmatrix_trans(pack_h2(p[n][0] - half_lo(h0), p[n][1] - half_hi(h0)));
-          bl1[n] = movmatrix_trans(pack_h2(p[n][2] - half_lo(h1), p[n][3] - half_hi(h1)));
-        }
-      }
-      {  // z + 8 s: row g is group g, row g + 8 (PREC > 0) what its fp16 value leaves
-        // (rows past G are not used)
-        const unsigned short* x = reinterpret_cast<const unsigned short*>(vsc + rt * S::kScaleRow) + g % G;
-        constexpr int kNext = S::kScaleRow / 2;
-        uint32_t za = __byte_perm(x[G], x[G + kNext], 0x5410), la = 0;
-        uint32_t zb = __byte_perm(x[G + 8 * kNext], x[G + 9 * kNext], 0x5410), lb = 0;
-        const uint32_t ta = __byte_perm(x[0], x[kNext], 0x5410), tb = __byte_perm(x[8 * kNext], x[9 * kNext], 0x5410);
-        if constexpr (PREC > 0) {
-          centre_zero(za, la, ta, z_unit);
-          centre_zero(zb, lb, tb, z_unit);
-        } else {
-          const uint32_t one = z_unit == 1.f ? 0x3c003c00u : 0x2c002c00u, eight = z_unit == 1.f ? 0x48004800u : 0x38003800u;
-          za = hfma2_u(ta, eight, hmul2_u(za, one));
-          zb = hfma2_u(tb, eight, hmul2_u(zb, one));
+      for (int i = 0; i < (G + 1) / 2; ++i) most = __vmaxu2(most, vtop[i]);
+      most = max(most & 0xffffu, most >> 16);
+      if (__any_sync(0xffffffffu, up || most > top)) {
+        float shrink = 1.f;
+        const uint32_t all = min(__reduce_max_sync(0xffffffffu, most), 0x7bffu);
+        if (all > top) {
+          const uint32_t to = (all + 0x3ffu) & 0x7c00u;  // the next power of two
+          shrink = __uint_as_float((127u - ((to - top) >> 10)) << 23);
+          unit2 -= static_cast<float>((to - top) >> 10);
+          if (to > kWide && top <= kWide) {
+            z_unit = 0.0625f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) zo[n][e] *= z_unit;
+          }
+          top = to;
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          mma_f16(zo[n], za, la, zb, lb, b0[n], b1[n]);
-          if constexpr (PREC > 0) mma_f16(zo[n], za, la, zb, lb, bl0[n], bl1[n]);
+          float f[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float x = mn[n][c];
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
+            x = fmaxf(m[n][c], x);
+            // nothing seen yet: 0, not exp2(-inf + inf)
+            f[c] = m[n][c] == -INFINITY ? 0.f : fast_exp2((m[n][c] - x) * q_unit[n][c]) * shrink;
+            l[n][c] *= f[c];
+            m[n][c] = x;
+            limit[n][c] = x + kSlack / q_unit[n][c];
+            base2[n][c] = x == -INFINITY ? unit2 : fmaf(-x, q_unit[n][c], unit2);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) zo[n][e] *= f[e & 1];
+#pragma unroll
+          for (int j = 0; j < G; ++j)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[n][j][u][e] *= f[e & 1];
         }
       }
-      uint32_t sa[(G + 1) / 2], sb[(G + 1) / 2], sd[(G + 1) / 2], se[(G + 1) / 2];
-      if constexpr (PREC == 0) {
-        lds_words<2 * G>(vsc + rt * S::kScaleRow, sa);
-        lds_words<2 * G>(vsc + (rt + 1) * S::kScaleRow, sb);
-        lds_words<2 * G>(vsc + (rt + 8) * S::kScaleRow, sd);
-        lds_words<2 * G>(vsc + (rt + 9) * S::kScaleRow, se);
-      } else {
-        lds_words<2 * G>(vsc + (hh * 16 + g) * S::kScaleRow, sa);
-        lds_words<2 * G>(vsc + (hh * 16 + g + 8) * S::kScaleRow, sb);
-      }
-      const auto group = [&](auto jc) {
-        constexpr int j = decltype(jc)::value;
-        uint32_t x0[4], x1[4];
-        nibbles<true>(pair16<j, j>(v0, v1), x0);
-        nibbles<true>(pair16<j, j>(v2, v3), x1);
+      // ---- P V
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        float p[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            p[n][e] = fast_exp2(fmaf(sc[hh][n][e], q_unit[n][e & 1], base2[n][e & 1]));
+            l[n][e & 1] += p[n][e];
+          }
+        const int rt = hh * 16 + 2 * t;  // this lane's tokens in the product: rt, rt+1, rt+8, rt+9
+        uint32_t v0[(G + 1) / 2], v1[(G + 1) / 2], v2[(G + 1) / 2], v3[(G + 1) / 2];
+        const unsigned char* vr = vs + hh * 16 * S::kRow;
+        lds_words<2 * G>(vr + v_at, v0);
+        lds_words<2 * G>(vr + v_at1, v1);
+        lds_words<2 * G>(vr + 8 * S::kRow + v_at, v2);
+        lds_words<2 * G>(vr + 8 * S::kRow + v_at1, v3);
+        uint32_t b0[NT], b1[NT], bl0[NT], bl1[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          if constexpr (PREC == 0) {
-            const uint32_t y0 = hmul2_u(b0[n], pair16<j, j>(sa, sb)), y1 = hmul2_u(b1[n], pair16<j, j>(sd, se));
-            mma_f16(o[n][j][0], x0[0], x0[1], x1[0], x1[1], y0, y1);
-            mma_f16(o[n][j][1], x0[2], x0[3], x1[2], x1[3], y0, y1);
-          } else {
-            const float f0 = j & 1 ? half_hi(sa[j / 2]) : half_lo(sa[j / 2]);
-            const float f1 = j & 1 ? half_hi(sb[j / 2]) : half_lo(sb[j / 2]);
-            const float y[4] = {p[n][0] * f0, p[n][1] * f0, p[n][2] * f1, p[n][3] * f1};
-            const uint32_t h0 = pack_h2(y[0], y[1]), h1 = pack_h2(y[2], y[3]);
-            const uint32_t y0 = movmatrix_trans(h0), y1 = movmatrix_trans(h1);
-            const uint32_t u0 = movmatrix_trans(pack_h2(y[0] - half_lo(h0), y[1] - half_hi(h0)));
-            const uint32_t u1 = movmatrix_trans(pack_h2(y[2] - half_lo(h1), y[3] - half_hi(h1)));
-            mma_f16(o[n][j][0], x0[0], x0[1], x1[0], x1[1], y0, y1);
-            mma_f16(o[n][j][1], x0[2], x0[3], x1[2], x1[3], y0, y1);
-            mma_f16(o[n][j][0], x0[0], x0[1], x1[0], x1[1], u0, u1);
-            mma_f16(o[n][j][1], x0[2], x0[3], x1[2], x1[3], u0, u1);
+          const uint32_t h0 = pack_h2(p[n][0], p[n][1]), h1 = pack_h2(p[n][2], p[n][3]);
+          b0[n] = movmatrix_trans(h0);
+          b1[n] = movmatrix_trans(h1);
+          if constexpr (PREC > 0) {
+            bl0[n] = movmatrix_trans(pack_h2(p[n][0] - half_lo(h0), p[n][1] - half_hi(h0)));
+            bl1[n] = movmatrix_trans(pack_h2(p[n][2] - half_lo(h1), p[n][3] - half_hi(h1)));
           }
         }
-      };
-      for_each_index(group, std::make_integer_sequence<int, G>{});
+        {  // z + 8 s: row g is group g, row g + 8 (PREC > 0) what its fp16 value leaves
+          // (rows past G are not used)
+          const unsigned short* x = reinterpret_cast<const unsigned short*>(vsc + rt * S::kScaleRow) + g % G;
+          constexpr int kNext = S::kScaleRow / 2;
+          uint32_t za = __byte_perm(x[G], x[G + kNext], 0x5410), la = 0;
+          uint32_t zb = __byte_perm(x[G + 8 * kNext], x[G + 9 * kNext], 0x5410), lb = 0;
+          const uint32_t ta = __byte_perm(x[0], x[kNext], 0x5410), tb = __byte_perm(x[8 * kNext], x[9 * kNext], 0x5410);
+          if constexpr (PREC > 0) {
+            centre_zero(za, la, ta, z_unit);
+            centre_zero(zb, lb, tb, z_unit);
+          } else {
+            const uint32_t one = z_unit == 1.f ? 0x3c003c00u : 0x2c002c00u, eight = z_unit == 1.f ? 0x48004800u : 0x38003800u;
+            za = hfma2_u(ta, eight, hmul2_u(za, one));
+            zb = hfma2_u(tb, eight, hmul2_u(zb, one));
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_f16(zo[n], za, la, zb, lb, b0[n], b1[n]);
+            if constexpr (PREC > 0) mma_f16(zo[n], za, la, zb, lb, bl0[n], bl1[n]);
+          }
+        }
+        uint32_t sa[(G + 1) / 2], sb[(G + 1) / 2], sd[(G + 1) / 2], se[(G + 1) / 2];
+        if constexpr (PREC == 0) {
+          lds_words<2 * G>(vsc + rt * S::kScaleRow, sa);
+          lds_words<2 * G>(vsc + (rt + 1) * S::kScaleRow, sb);
+          lds_words<2 * G>(vsc + (rt + 8) * S::kScaleRow, sd);
+          lds_words<2 * G>(vsc + (rt + 9) * S::kScaleRow, se);
+        } else {
+          lds_words<2 * G>(vsc + (hh * 16 + g) * S::kScaleRow, sa);
+          lds_words<2 * G>(vsc + (hh * 16 + g + 8) * S::kScaleRow, sb);
+        }
+        const auto group = [&](auto jc) {
+          constexpr int j = decltype(jc)::value;
+          uint32_t x0[4], x1[4];
+          nibbles<true>(pair16<j, j>(v0, v1), x0);
+          nibbles<true>(pair16<j, j>(v2, v3), x1);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            if constexpr (PREC == 0) {
+              const uint32_t y0 = hmul2_u(b0[n], pair16<j, j>(sa, sb)), y1 = hmul2_u(b1[n], pair16<j, j>(sd, se));
+              mma_f16(o[n][j][0], x0[0], x0[1], x1[0], x1[1], y0, y1);
+              mma_f16(o[n][j][1], x0[2], x0[3], x1[2], x1[3], y0, y1);
+            } else {
+              const float f0 = j & 1 ? half_hi(sa[j / 2]) : half_lo(sa[j / 2]);
+              const float f1 = j & 1 ? half_hi(sb[j / 2]) : half_lo(sb[j / 2]);
+              const float y[4] = {p[n][0] * f0, p[n][1] * f0, p[n][2] * f1, p[n][3] * f1};
+              const uint32_t h0 = pack_h2(y[0], y[1]), h1 = pack_h2(y[2], y[3]);
+              const uint32_t y0 = movmatrix_trans(h0), y1 = movmatrix_trans(h1);
+              const uint32_t u0 = movmatrix_trans(pack_h2(y[0] - half_lo(h0), y[1] - half_hi(h0)));
+              const uint32_t u1 = movmatrix_trans(pack_h2(y[2] - half_lo(h1), y[3] - half_hi(h1)));
+              mma_f16(o[n][j][0], x0[0], x0[1], x1[0], x1[1], y0, y1);
+              mma_f16(o[n][j][1], x0[2], x0[3], x1[2], x1[3], y0, y1);
+              mma_f16(o[n][j][0], x0[0], x0[1], x1[0], x1[1], u0, u1);
+              mma_f16(o[n][j][1], x0[2], x0[3], x1[2], x1[3], u0, u1);
+            }
+          }
+        };
+        for_each_index(group, std::make_integer_sequence<int, G>{});
+      }
+      stage = stage == ST - 1 ? 0 : stage + 1;
     }
-    stage = stage == ST - 1 ? 0 : stage + 1;
-  }
 
-  // ---- merge the warps (the ring is free once every copy has landed)
-  cp_async_wait<0>();
-  __syncthreads();
-  constexpr int kLd = D + 4;  // row: D outputs, the maximum, the sum
-  float* buf = reinterpret_cast<float*>(i4_smem);
-  const float one = exp2f(-unit2);
+    // ---- merge the warps (the ring is free once every copy has landed)
+    cp_async_wait<0>();
+    __syncthreads();
+    constexpr int kLd = D + 4;  // row: D outputs, the maximum, the sum
+    float* buf = reinterpret_cast<float*>(i4_smem);
+    const float one = exp2f(-unit2);
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float s = l[n][c];
+      for (int c = 0; c < 2; ++c) {
+        float s = l[n][c];
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-      float* row = buf + (warp * HN + n * 8 + 2 * t + c) * kLd;
-      if (g == 0) row[D] = m[n][c] == -INFINITY ? -INFINITY : m[n][c] * q_unit[n][c], row[D + 1] = s * one;
+        for (int off = 4; off < 32; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        float* row = buf + (warp * HN + n * 8 + 2 * t + c) * kLd;
+        if (g == 0) row[D] = m[n][c] == -INFINITY ? -INFINITY : m[n][c] * q_unit[n][c], row[D + 1] = s * one;
 #pragma unroll
-      for (int j = 0; j < G; ++j) {
-        const float z = __shfl_sync(0xffffffffu, zo[n][c] + zo[n][2 + c], j * 4 + t) * (1.f / z_unit);
+        for (int j = 0; j < G; ++j) {
+          const float z = __shfl_sync(0xffffffffu, zo[n][c] + zo[n][2 + c], j * 4 + t) * (1.f / z_unit);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          *reinterpret_cast<float2*>(row + 32 * j + 4 * g + 2 * u) =
-              make_float2((o[n][j][u][c] + z) * one, (o[n][j][u][2 + c] + z) * one);
+          for (int u = 0; u < 2; ++u)
+            *reinterpret_cast<float2*>(row + 32 * j + 4 * g + 2 * u) =
+                make_float2((o[n][j][u][c] + z) * one, (o[n][j][u][2 + c] + z) * one);
+        }
       }
     }
-  }
-  merge_warps<W, HN, D>(a, seg, q0, heads, buf, s_f);
-  __syncthreads();  // the next segment's loads reuse the buffer
+    merge_warps<W, HN, D>(a, seg, q0, heads, buf, s_f);
+    __syncthreads();  // the next segment's loads reuse the buffer
   }
 }
 
