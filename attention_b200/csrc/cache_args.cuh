@@ -142,11 +142,18 @@ __device__ __forceinline__ void split_range(int n, int split, int nsplit, int& t
 }
 
 // ---- Sharing out the work.  A pair is a (sequence, kv head, chunk of its query heads); all of a
-// sequence's pairs have its number of tiles.  The pairs' tiles, end to end, are cut into `ctas`
-// equal ranges, one a CTA, however the lengths are spread; a range may end inside a pair, so a
+// sequence's pairs have its number of tiles.  The pairs' tiles, end to end, are cut into
+// sharing_ctas() equal ranges, one a CTA, however the lengths are spread; a range may end inside a pair, so a
 // pair's results are partials of consecutive CTAs, in slot CTA + pair (both only ever grow along
 // the ranges, so no two share a slot).  A pair that one CTA covers whole needs no partial.
 constexpr int kFlatBatch = 1024;  // longest batch whose prefix sums a CTA makes for itself
+
+// The launch has a.ctas CTAs, planned from the room that the contexts may grow into; where there
+// are fewer tiles than that, as many CTAs as tiles share them and the others do nothing.  Every
+// range then holds a tile, so every CTA between a pair's first and last has left a partial.
+__device__ __forceinline__ int sharing_ctas(const CacheDecodeArgs& a, int64_t total) {
+  return total < a.ctas ? static_cast<int>(total) : a.ctas;
+}
 
 // pre[b] = tiles of one pair of each sequence before b, pre[B] the total; every thread calls it.
 template <int TILE>
@@ -193,9 +200,16 @@ struct Segment {
 struct Work {
   int64_t x, x1;
   __device__ __forceinline__ Work(const CacheDecodeArgs& a, const int* pre) {
-    const int64_t total = static_cast<int64_t>(a.ctas ? pre[a.B] : 0) * a.Hkv * a.chunks;
-    x = a.ctas ? mul_div(total, blockIdx.x, a.ctas) : 0;
-    x1 = a.ctas ? mul_div(total, blockIdx.x + 1, a.ctas) : 1;
+    x = 0, x1 = 1;
+    if (!a.ctas) return;
+    const int64_t total = static_cast<int64_t>(pre[a.B]) * a.Hkv * a.chunks;
+    const int ctas = sharing_ctas(a, total), i = blockIdx.x;
+    if (i >= ctas) {
+      x1 = 0;
+      return;
+    }
+    x = mul_div(total, i, ctas);
+    x1 = mul_div(total, i + 1, ctas);
   }
   template <int TILE>
   __device__ __forceinline__ bool next(const CacheDecodeArgs& a, const int* pre, Segment& s) {
@@ -233,7 +247,7 @@ struct Work {
     return true;
   }
 };
-// CTAs [first, last] that hold tiles [at, at + n) of all `total`, n > 0
+// CTAs [first, last] of `ctas` <= total that hold tiles [at, at + n) of all `total`, n > 0
 __device__ __forceinline__ void ctas_of(int64_t at, int n, int64_t total, int ctas, int& first, int& last) {
   // the last CTA whose range starts at or before tile x: the largest i with total i / ctas <= x
   const auto cta = [&](int64_t x) {
