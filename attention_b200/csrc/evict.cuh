@@ -200,8 +200,8 @@ __global__ void __launch_bounds__(kSelThreads, 4) select_tokens_kernel(const flo
 // chunk after that (keep, then the page table) are being looked up, once a row.
 //
 // Bound by HBM (each kept row read and written once) and the cluster's rounds: 64 pairs, 8192 of
-// 32768 rows of 256 bytes take 123 us, 0.69 of the copy bandwidth (777 us with one CTA a pool
-// and pair, 137 with both look-ups of a row in one step).
+// 32768 rows of 256 bytes take 133 us, 0.63 of the copy bandwidth (777 us with one CTA a pool
+// and pair; with the next chunk's arrival before this one's stores 152).
 constexpr int kMaxPools = 8;
 struct CompactArgs {
   unsigned char* pool[kMaxPools];
@@ -313,22 +313,9 @@ __device__ __forceinline__ void compact_rows(U* pool, int rows, int per, int ran
         if (r.y >= 0) pool[r.y * per + off_of[u]] = v[k][u];
       }
   };
-  // The loads have returned before the cluster is told that they have: that orders them before
-  // the others' stores, so the arrival needs no fence (which would wait for the last chunk's
-  // stores).  The CTA barrier after the wait orders the tables.
-  const auto arrive = [&](int k) {
-#pragma unroll
-    for (int u = 0; u < kCompactUnroll; ++u) {
-      if constexpr (sizeof(U) >= 4) {
-#pragma unroll
-        for (int w = 0; w < static_cast<int>(sizeof(U)) / 4; ++w)
-          asm volatile("" ::"r"(reinterpret_cast<const uint32_t*>(&v[k][u])[w]) : "memory");
-      } else {
-        asm volatile("" ::"r"(static_cast<uint32_t>(v[k][u])) : "memory");
-      }
-    }
-    cluster_arrive_relaxed();
-  };
+  // A CTA's loads of a chunk come before every other CTA's stores of it: the arrival releases
+  // them (and waits for this CTA's earlier stores to be seen), the wait acquires.  That orders the
+  // tables as well.
   if (looks) {
     for (int c = 0; c < 2; ++c) {
       first(c);
@@ -349,10 +336,9 @@ __device__ __forceinline__ void compact_rows(U* pool, int rows, int per, int ran
         at.second();
         first(c + k + 4);
       }
-      arrive(k);
+      cluster_arrive();
       if (c + k + 1 < chunks) load(c + k + 1, 1 - k);
       cluster_wait();
-      __syncthreads();
       if (c + k < chunks) store(c + k, k);
     }
   }
