@@ -397,6 +397,7 @@ __global__ void __launch_bounds__(kCompactThreads, kCompactCtas) compact_kernel(
   }
   if (which == 0 && a.weights) {
     float* w = a.weights + bh * a.T;
+    __syncthreads();  // the pool's last stores still read the tables that the weights' rows go into
     compact_rows(reinterpret_cast<uint32_t*>(w), n, 1, rank, ranks, s_rows, CompactWeights{keep});
     // the sources behind row n have all been loaded (an empty list had no chunk to wait for,
     // and no sources)

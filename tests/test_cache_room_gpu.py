@@ -127,3 +127,45 @@ def test_long_window_over_a_short_context(nan_workspaces, dtype, dim):
         # as in Roomy.check: Q < 2^7 for these sizes, D + 8 <= 168
         tol = (2 * 168 * 2.0 ** -24 * 2 ** 7 + 2.0 ** -10) * 3 * cache.values[1].abs().max()
         assert ((out.double().cpu() - want).abs() <= tol + torch.finfo(dtype).eps / 2 * want.abs()).all()
+
+
+@pytest.mark.parametrize("kind", ["int4", "bf16"])
+def test_serving_loop_grows_into_its_room(nan_workspaces, kind):
+    """A prompt of 20 tokens in a table of 2048, prompts appended turn by turn, a step with weights after each,
+    and an eviction: every output against a 64-bit model."""
+    gen = torch.Generator().manual_seed(3)
+    batch, dim, room, budget, recent = 2, 64, 2048, 300, 40
+    dt = torch.bfloat16
+    pages = room // PAGE
+    make = spa.PagedKVCacheInt4 if kind == "int4" else spa.PagedKVCache
+    cache = make(batch * pages, HEADS, PAGE, dim, batch=batch, max_pages_per_seq=pages)
+    cache.page_table.copy_(torch.randperm(batch * pages, generator=gen).view(batch, pages).to(torch.int32))
+    stored = (lambda x: ref.int4_dequantise(ref.int4_quantise(x))) if kind == "int4" else (lambda x: x.double())
+    decode = spa.paged_decode_attention_int4 if kind == "int4" else spa.paged_decode_attention
+    w = torch.zeros(batch, HEADS, room, device=DEV)
+    model = [torch.zeros(batch, HEADS, 0, dim, dtype=torch.float64) for _ in range(2)]
+    acc = torch.zeros(batch, HEADS, 0, dtype=torch.float64)
+    for turn in (20, 1, 70, 400, 1, 200, 30):
+        new = [torch.randn(batch, HEADS, turn, dim, generator=gen).to(dt) for _ in range(2)]
+        if kind == "int4":
+            spa.kv_append_int4(cache.k, cache.v, cache.page_table, *(x.to(DEV) for x in new), cache.context_lens)
+        else:
+            for t in range(turn):
+                spa.kv_append(cache.k, cache.v, cache.page_table, *(x[:, :, t].to(DEV) for x in new),
+                              cache.context_lens + t)
+        cache.context_lens += turn
+        model = [torch.cat((m, stored(x)), 2) for m, x in zip(model, new)]
+        q = torch.randn(batch, HEADS * GROUP, dim, generator=gen).to(dt)
+        out = decode(q.to(DEV), cache.k, cache.v, page_table=cache.page_table, context_lens=cache.context_lens, weights=w)
+        n = model[0].size(2)
+        want, ww = ref.attention_weights(q, *model, [torch.arange(n)] * batch)
+        acc = torch.nn.functional.pad(acc, (0, turn)) + ww
+        # scores of these sizes are off by under 2^-12, P by 2^-10, the output by half a bf16 step
+        assert ((out.double().cpu() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -9 * model[1].abs().max() * 3).all()
+        got = w.double().cpu()
+        assert ((got[..., :n] - acc).abs() <= 2.0 ** -11 * acc).all() and (got[..., n:] == 0).all()
+        if n > 600:
+            keep = spa.evict_tokens(cache, w, budget=budget, recent=recent).cpu().long()
+            assert torch.equal(keep.int(), ref.select_tokens(got.float(), [n] * batch, budget, recent)[0])
+            model = [m.gather(2, keep[..., None].expand(-1, -1, -1, dim)) for m in model]
+            acc = acc.gather(2, keep)

@@ -69,3 +69,47 @@ def test_rows_of_every_unit(row):
     want = moved(pool, table, keep)
     spa.compact_tokens((pool,), table, keep)
     assert torch.equal(pool, want)
+
+
+# of 128 bytes (128 rows a chunk of a CTA) or 256 (64): 2, 6 and 10 chunks end on the table that the
+# weights' rows go into first
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("chunks", [1, 2, 4, 6, 10])
+def test_weights_follow_the_rows(dim, chunks):
+    gen = torch.Generator(device=DEV).manual_seed(chunks)
+    batch, heads, page = 2, 4, 32
+    budget = 8 * (8192 // dim) * chunks - 3
+    tokens = budget + 500
+    pages = -(-tokens // page)
+    for _ in range(8):
+        table = torch.randperm(batch * pages, generator=gen, device=DEV).view(batch, pages).int()
+        pools = [torch.randint(-2 ** 15, 2 ** 15, (batch * pages, heads, page, dim), generator=gen, device=DEV,
+                               dtype=torch.int16).view(torch.bfloat16) for _ in range(2)]
+        w = torch.rand(batch, heads, tokens, generator=gen, device=DEV)
+        keep = lists(batch, heads, budget, tokens, gen)
+        want = [moved(p.view(torch.int16), table, keep) for p in pools]
+        want_w = torch.zeros_like(w)
+        want_w[..., :budget] = w.gather(2, keep.long())
+        spa.compact_tokens(pools, table, keep, weights=w)
+        for p, x in zip(pools, want):
+            assert torch.equal(p.view(torch.int16), x)
+        assert torch.equal(w, want_w)
+
+
+def test_lists_of_unlike_lengths():
+    """Empty lists among long ones, with weights: their clusters have no chunk at all."""
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    batch, heads, page, dim, budget, tokens = 3, 4, 16, 64, 2048, 2500
+    pages = -(-tokens // page)
+    table = torch.randperm(batch * pages, generator=gen, device=DEV).view(batch, pages).int()
+    pool = torch.randint(0, 256, (batch * pages, heads, page, dim), generator=gen, device=DEV, dtype=torch.uint8)
+    w = torch.rand(batch, heads, tokens, generator=gen, device=DEV)
+    keep = lists(batch, heads, budget, tokens, gen)
+    for b, h, n in ((0, 0, 0), (0, 1, 1), (1, 0, 1024), (1, 2, 0), (2, 3, 1025)):
+        keep[b, h, n:] = -1
+    to = torch.arange(budget, device=DEV, dtype=torch.int32)
+    want = moved(pool, table, torch.where(keep >= 0, keep, to))
+    want_w = torch.zeros_like(w)
+    want_w[..., :budget] = torch.where(keep >= 0, w.gather(2, keep.long().clamp(min=0)), 0.0)
+    spa.compact_tokens((pool,), table, keep, weights=w)
+    assert torch.equal(pool, want) and torch.equal(w, want_w)
