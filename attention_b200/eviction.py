@@ -69,7 +69,8 @@ def compact_tokens(pools, page_table: torch.Tensor, keep: torch.Tensor, *,
             raise ValueError("pools must be [pages, Hkv, P, ...] of one geometry")
         if not t.is_contiguous():
             raise ValueError("contiguous CUDA tensors are required")
-        ptrs[i], sizes[i] = t.data_ptr(), t.stride(2) * t.element_size()
+        # (not stride(2): a contiguous tensor may have any stride there when P is 1)
+        ptrs[i], sizes[i] = t.data_ptr(), t.numel() // (shape[0] * shape[1] * shape[2]) * t.element_size()
     if page_table.get_device() != dev:
         raise ValueError("tensors must be on one device")
     if keep.dtype != torch.int32 or keep.dim() != 3 or keep.numel() == 0 or not keep.is_contiguous():

@@ -113,3 +113,17 @@ def test_lists_of_unlike_lengths():
     want_w[..., :budget] = torch.where(keep >= 0, w.gather(2, keep.long().clamp(min=0)), 0.0)
     spa.compact_tokens((pool,), table, keep, weights=w)
     assert torch.equal(pool, want) and torch.equal(w, want_w)
+
+
+def test_pages_of_one_token():
+    """A pool [pages, Hkv, 1, D] made by a transposition is contiguous with any stride for its third
+    dimension: the rows' size comes from the shape."""
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    batch, heads, dim, tokens, budget = 2, 3, 24, 90, 40
+    table = torch.randperm(batch * tokens, generator=gen, device=DEV).view(batch, tokens).int()
+    pool = torch.randn(batch * tokens, 1, heads, dim, generator=gen, device=DEV).transpose(1, 2)
+    assert pool.is_contiguous() and pool.stride(2) != dim
+    keep = lists(batch, heads, budget, tokens, gen)
+    want = moved(pool, table, keep)
+    spa.compact_tokens((pool,), table, keep)
+    assert torch.equal(pool, want)
