@@ -450,6 +450,10 @@ extern "C" int spa_compact_tokens(const spa_kv_layout* kv, int n_pools, void* co
     a.row_bytes[i] = row_bytes[i];
     const uintptr_t x = reinterpret_cast<uintptr_t>(pools[i]) | static_cast<uintptr_t>(row_bytes[i]);
     a.unit[i] = x % 16 == 0 ? 16 : x % 8 == 0 ? 8 : x % 4 == 0 ? 4 : x % 2 == 0 ? 2 : 1;
+    // clusters of their own move the pools side by side: none may share memory with another
+    for (int j = 0; j < i; ++j)
+      if (a.pool[i] < a.pool[j] + kv->total_rows * row_bytes[j] && a.pool[j] < a.pool[i] + kv->total_rows * row_bytes[i])
+        return SPA_ERR_INVALID;
   }
   a.n_pools = n_pools;
   a.addr = make_kv_addr(*kv);

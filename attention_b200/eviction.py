@@ -53,7 +53,7 @@ def compact_tokens(pools, page_table: torch.Tensor, keep: torch.Tensor, *,
     ``select_tokens`` returns it); a list that is not leaves its (sequence, kv head) as it was
     and raises the device error word.  ``weights`` ``[B, Hkv, T]`` move along and become zero
     behind the kept tokens; pool rows behind them stay as they were.  A page may belong to one
-    sequence only."""
+    sequence only, and no two pools may share memory (ValueError)."""
     flat = [t for p in pools for t in (p if isinstance(p, (tuple, list)) else (p,))]
     if not flat or len(flat) > 8:
         raise ValueError("pools must hold 1 to 8 tensors")

@@ -806,7 +806,7 @@ int spa_paged_decode_weights(const void* q, int dtype, int batch, int q_heads, i
  *
  * spa_compact_tokens: moves row keep[j] to token j, j = 0, 1, ..., in place, in each of the
  * n_pools (up to 8) pools; row_bytes[i] is the size of a row of pools[i], addressed by kv's
- * geometry (its k and v are not used).  weights, when given, move along and are zero behind
+ * geometry (its k and v are not used).  Pools that overlap are refused.  weights, when given, move along and are zero behind
  * the kept tokens.  Rows of the pools behind the kept tokens stay as they were.  keep must be
  * ascending and then -1, with no token twice; a (sequence, kv head) whose list is not is left
  * as it was and raises device error bit 4.  A row without a page is left out (bit 2).
