@@ -389,10 +389,11 @@ __global__ void __launch_bounds__(Int4Cfg<G, NT>::kWarps * 32, Int4Cfg<G, NT>::k
     // halves of those, over the widest range.
     uint32_t top = 0x3c00u;
     float unit2 = kUnit2;
-    // z + 8 s is held as it is, or, once scales above kWide = 4096 turned up (it might pass fp16's
-    // range), in sixteenths
-    constexpr uint32_t kWide = 0x6c00u;
+    // z + 8 s is held as it is, or, once scales above kWide = 4096 or zeros above kHigh = 28672 turned
+    // up (it might pass fp16's range), in sixteenths.  Zeros are compared as signed numbers.
+    constexpr uint32_t kWide = 0x6c00u, kHigh = 0x77007700u;
     float z_unit = 1.f;
+    uint32_t high = kHigh;  // fp16's NaN, which nothing is above, once z_unit is a sixteenth
 
     int stage = 0;
 #pragma unroll 1
@@ -408,11 +409,12 @@ __global__ void __launch_bounds__(Int4Cfg<G, NT>::kWarps * 32, Int4Cfg<G, NT>::k
       float sc[2][NT][4], mn[NT][2];
       float zk_unit = 1.f;  // as z_unit, for this tile of K
       if constexpr (kCentreK) {
-        uint32_t ktop[(G + 1) / 2], most = 0;
+        uint32_t ktop[(G + 1) / 2], kzero[(G + 1) / 2], most = 0, zero = kHigh;
         lds_words<2 * G>(ksc + lane * S::kScaleRow, ktop);
+        lds_words<2 * G>(ksc + lane * S::kScaleRow + 2 * G, kzero);
 #pragma unroll
-        for (int i = 0; i < (G + 1) / 2; ++i) most = __vmaxu2(most, ktop[i]);
-        if (__any_sync(0xffffffffu, max(most & 0xffffu, most >> 16) > kWide)) zk_unit = 0.0625f;
+        for (int i = 0; i < (G + 1) / 2; ++i) most = __vmaxu2(most, ktop[i]), zero = __vmaxs2(zero, kzero[i]);
+        if (__any_sync(0xffffffffu, max(most & 0xffffu, most >> 16) > kWide || zero != kHigh)) zk_unit = 0.0625f;
       }
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
@@ -521,27 +523,30 @@ __global__ void __launch_bounds__(Int4Cfg<G, NT>::kWarps * 32, Int4Cfg<G, NT>::k
           mn[n][c] = fmaxf(fmaxf(sc[0][n][c], sc[0][n][2 + c]), fmaxf(sc[1][n][c], sc[1][n][2 + c]));
           up |= mn[n][c] > limit[n][c];
         }
-      // largest V scale of the tile: this lane's token (NaN and negative ones count as fp16's largest)
-      uint32_t vtop[(G + 1) / 2], most = 0;
+      // largest V scale and zero of the tile: this lane's token (NaN and negative scales count as
+      // fp16's largest)
+      uint32_t vtop[(G + 1) / 2], vzero[(G + 1) / 2], most = 0, zero = high;
       lds_words<2 * G>(vsc + lane * S::kScaleRow, vtop);
+      lds_words<2 * G>(vsc + lane * S::kScaleRow + 2 * G, vzero);
 #pragma unroll
-      for (int i = 0; i < (G + 1) / 2; ++i) most = __vmaxu2(most, vtop[i]);
+      for (int i = 0; i < (G + 1) / 2; ++i) most = __vmaxu2(most, vtop[i]), zero = __vmaxs2(zero, vzero[i]);
       most = max(most & 0xffffu, most >> 16);
-      if (__any_sync(0xffffffffu, up || most > top)) {
+      if (__any_sync(0xffffffffu, up || most > top || zero != high)) {
         float shrink = 1.f;
         const uint32_t all = min(__reduce_max_sync(0xffffffffu, most), 0x7bffu);
         if (all > top) {
           const uint32_t to = (all + 0x3ffu) & 0x7c00u;  // the next power of two
           shrink = __uint_as_float((127u - ((to - top) >> 10)) << 23);
           unit2 -= static_cast<float>((to - top) >> 10);
-          if (to > kWide && top <= kWide) {
-            z_unit = 0.0625f;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) zo[n][e] *= z_unit;
-          }
           top = to;
+        }
+        if (z_unit == 1.f && (top > kWide || __any_sync(0xffffffffu, zero != high))) {
+          z_unit = 0.0625f;
+          high = 0x7fff7fffu;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) zo[n][e] *= z_unit;
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
