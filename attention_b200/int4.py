@@ -155,9 +155,11 @@ def check_weights(weights, batch: int, kv_heads: int, dev: int) -> None:
 
 
 @functools.lru_cache(maxsize=256)
-def cache_decode_workspace(*shape) -> int:
-    """``spa_cache_decode_workspace_size``, a function of the shape alone."""
-    return _lib.lib.spa_cache_decode_workspace_size(*shape)
+def cache_decode_workspace(device: int, *shape) -> int:
+    """``spa_cache_decode_workspace_size`` on CUDA device ``device``: a function of the shape and
+    of the device's number of SMs."""
+    with torch.cuda.device(device):
+        return _lib.lib.spa_cache_decode_workspace_size(*shape)
 
 
 def _decode(query, k_pool, v_pool, page_table, context_lens, local_window, selected, weights, block_size=None):
@@ -192,7 +194,7 @@ def _decode(query, k_pool, v_pool, page_table, context_lens, local_window, selec
     out = torch.empty_like(query)
     if batch == 0:
         return out
-    need = cache_decode_workspace(batch, q_heads, kv_heads, dim, most, tokens, w_ptr is not None, -1)
+    need = cache_decode_workspace(dev, batch, q_heads, kv_heads, dim, most, tokens, w_ptr is not None, -1)
     # from the caching allocator, per call: ordered with the stream, and a captured graph keeps its own
     ws = torch.empty(need, dtype=torch.uint8, device=table.device) if need else None
     rc = launch(_lib.lib.spa_int4_decode, dev, query.data_ptr(), code, batch, q_heads, kv_heads, dim,

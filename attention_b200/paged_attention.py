@@ -75,7 +75,7 @@ def _decode_weights(query, layout, kv_heads, lens, tokens, local_window, max_can
         raise ValueError("tensors must be on one device")
     out = torch.empty_like(query)
     code = dtype_code(query)
-    need = cache_decode_workspace(batch, q_heads, kv_heads, head_dim, max_candidates, tokens, 1, code)
+    need = cache_decode_workspace(dev, batch, q_heads, kv_heads, head_dim, max_candidates, tokens, 1, code)
     ws = torch.empty(need, dtype=torch.uint8, device=query.device)
     rc = launch(_lib.lib.spa_paged_decode_weights, dev, query.data_ptr(), code, batch, q_heads, kv_heads, head_dim,
                 ctypes.byref(layout), lens.data_ptr(), tokens, local_window, max_candidates, head_dim ** -0.5,
