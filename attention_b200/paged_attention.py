@@ -75,6 +75,8 @@ def _decode_weights(query, layout, kv_heads, lens, tokens, local_window, max_can
         raise ValueError("tensors must be on one device")
     out = torch.empty_like(query)
     code = dtype_code(query)
+    if batch == 0:
+        return out
     need = cache_decode_workspace(dev, batch, q_heads, kv_heads, head_dim, max_candidates, tokens, 1, code)
     ws = torch.empty(need, dtype=torch.uint8, device=query.device)
     rc = launch(_lib.lib.spa_paged_decode_weights, dev, query.data_ptr(), code, batch, q_heads, kv_heads, head_dim,
