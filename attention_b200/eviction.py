@@ -95,7 +95,8 @@ def compact_tokens(pools, page_table: torch.Tensor, keep: torch.Tensor, *,
 def evict_tokens(cache, weights: torch.Tensor, *, budget: int, recent: int) -> torch.Tensor:
     """Cuts every sequence of a ``PagedKVCache`` or ``PagedKVCacheInt4`` to ``budget`` tokens:
     ``select_tokens``, ``compact_tokens`` of K, V and ``weights``, and ``context_lens`` in
-    place.  Returns ``keep``.  Nothing synchronises, so the whole can be captured."""
+    place.  ``weights`` must cover the contexts, as decode asks (and reports): tokens past them
+    are dropped.  Returns ``keep``.  Nothing synchronises, so the whole can be captured."""
     if budget > weights.size(-1):
         raise ValueError("budget must not exceed the weights' tokens")
     keep, kept = select_tokens(weights, cache.context_lens, budget=budget, recent=recent)
