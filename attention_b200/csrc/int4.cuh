@@ -50,8 +50,8 @@ __device__ __forceinline__ int64_t int4_row(const Int4Rows& a, int b, int h, int
 //
 // Bound by HBM (a row's 2 D bytes against its 5/8 D at 16 bits) as long as a value costs few
 // instructions: 9 here to quantise one; with a group spread over 8 lanes and a division a value
-// it was 63.  4 prompts of up to 8192 tokens, 8 heads of 128 in bf16: 59 us for both kernels, 0.70
-// of the copy bandwidth (140 us that way).
+// it was 63.  4 prompts of up to 8192 tokens, 8 heads of 128 in bf16: 62 us for both kernels (the mean
+// of six draws of their lengths), 0.67 of the copy bandwidth (twice as long that way).
 constexpr int kInt4Warps = 4, kInt4Stretch = 32;
 
 // 32 consecutive values of a row as fp32; `vec` when 16-byte loads are allowed.

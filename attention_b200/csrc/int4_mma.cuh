@@ -16,20 +16,21 @@
 // of the PV product, the query heads of the kv head its 8 columns; the sum over a group's 32
 // values is a pair of k-steps, after which the scale is one fp32 multiply a score.  The zeros
 // go through one more product per 16 tokens, of z with the queries' group sums (held as two
-// halves).  For PV the scale goes into the probabilities: p s in fp16 for a bf16 output
-// (2 roundings of 2^-11 against the output's 2^-8), as two halves (22 bits) otherwise.
+// halves).  For PV the scale goes into the probabilities: p, p s and z + 8 s in fp16 for a bf16
+// output (roundings of 2^-11 against the output's 2^-8), as two halves (22 bits) otherwise.
 //
 // What bounds it: HBM, 160 bytes a token and kv head at D = 128, if the instructions keep up:
-// at 6.5 TB/s an SM has 2.8 issue slots per value, and a tile takes 2.6 a value.  Each warp
+// at 6.5 TB/s an SM has 3.5 issue slots per value, and a tile takes 2.6 a value.  Each warp
 // streams a stretch of tiles of 32 tokens (5 KB) through its own ring of cp.async stages in
 // shared memory, without barriers between warps, so pages of any size, order and alignment
 // cost the same.
 //
 // Measured (B200, 32 query and 8 kv heads of 128, bf16, pages of 128): 8 x 32768 tokens 76 us, 4.4
-// TB/s or 0.67 of the copy bandwidth; 8 x 131072 tokens 259 us, 0.79.  In long contexts what is
-// left is the instructions (IPC 2.3 of 4 with 12 warps an SM; with 16 warps of 128 registers it
-// was 80 us, with the maximum moved at every rise 90); some 12 us of every call are the phases
-// before the first product and after the last, and the joining kernel.
+// TB/s or 0.67 of the copy bandwidth; 8 x 131072 tokens 259 us, 0.79.  No pipe is full (IPC 2.4 of
+// 4, ALU 51 %, tensor 25 %) and few warps wait for memory: what is left, with 12 warps an SM, is
+// instructions that wait for the one before (with 16 warps of 128 registers it was 80 us, with the
+// maximum moved at every rise 90).  Some 12 us of every call are the phases before the first
+// product and after the last, and the joining kernel.
 #pragma once
 
 #include "cache_args.cuh"

@@ -10,7 +10,7 @@
 // Bound by HBM: 512 bytes a token and kv head at D = 128, and the scores (16 bytes written and read
 // at four query heads).  Each warp streams a stretch of tiles of 16 tokens (8 KB) through its own
 // ring of cp.async stages, three deep.  8 x 16384 tokens, 32 query and 8 kv heads of 128 in bf16:
-// 105 us with the weights' sum, 0.79 of the copy bandwidth (the CUDA-core kernel: 868 us).
+// 103 us with the weights' sum, 0.81 of the copy bandwidth (the CUDA-core kernel: 868 us).
 #pragma once
 
 #include "cache_args.cuh"
