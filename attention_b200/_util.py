@@ -64,12 +64,14 @@ def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
 
 
 def const_i32(device: torch.device, n: int, value: int) -> torch.Tensor:
-    """A cached int32 device vector of length n filled with value (read-only use)."""
+    """A cached int32 device vector of length n filled with value (read-only use).  One made while
+    a graph is captured is the graph's own, filled by its replays, and is not kept."""
     key = (device.index, n, value)
     t = _CONST_I32.get(key)
     if t is None:
         t = torch.full((n,), value, dtype=torch.int32, device=device)
-        _CONST_I32[key] = t
+        if not torch.cuda.is_current_stream_capturing():
+            _CONST_I32[key] = t
     return t
 
 

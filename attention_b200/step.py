@@ -132,8 +132,9 @@ def _prepared_step(query, keys, values, summaries, *, top_blocks, local_window, 
     borrowed = pr["summ"] is summaries and (super_summaries is None or sup is super_summaries) and (
         page_table is None or (pr["lens"] is context_lens and pr["layout"].page_table == page_table.data_ptr()
                                and page_table.dtype == torch.int32))
-    if not borrowed:
-        # converted copies: the arguments point into them, so the entry keeps them
+    if not borrowed or torch.cuda.is_current_stream_capturing():
+        # converted copies: the arguments point into them, so the entry keeps them; what was made
+        # during a capture is that graph's own, and only its replays fill it
         entry["keep"] = pr
         return entry
     _remember(_STEP_META, mkey, entry)
