@@ -25,6 +25,10 @@ def stream_ptr(device: torch.device | int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+# whether the current stream is being captured (torch.cuda.is_current_stream_capturing without its wrapper)
+is_capturing = torch._C._cuda_isCurrentStreamCapturing
+
+
 def launch(fn, device: int, *args) -> int:
     """Calls the C entry point ``fn(*args, stream)`` with CUDA device ``device`` current, on the
     caller's stream of that device."""
@@ -53,8 +57,11 @@ _CONST_I32: dict[tuple, torch.Tensor] = {}
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """A device byte buffer of at least ``nbytes`` reserved for the caller's current
     stream (one buffer per (device, stream); calls on one stream are ordered, so the
-    buffer is never used by two kernels at once).  The decode kernels write every
-    partial they read back, so no initial contents are needed."""
+    buffer is never used by two kernels at once).  A captured call gets memory of its graph:
+    graphs may be replayed side by side, on any stream, and after the buffer has grown.  The
+    decode kernels write every partial they read back, so no initial contents are needed."""
+    if is_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device.index, stream_ptr(device))
     buf = _WORKSPACES.get(key)
     if buf is None or buf.numel() < nbytes:
@@ -70,7 +77,7 @@ def const_i32(device: torch.device, n: int, value: int) -> torch.Tensor:
     t = _CONST_I32.get(key)
     if t is None:
         t = torch.full((n,), value, dtype=torch.int32, device=device)
-        if not torch.cuda.is_current_stream_capturing():
+        if not is_capturing():
             _CONST_I32[key] = t
     return t
 

@@ -24,7 +24,7 @@ import weakref
 import torch
 
 from . import _lib
-from ._util import as_int32, const_i32, dtype_code, stream_ptr, workspace
+from ._util import as_int32, const_i32, dtype_code, is_capturing, stream_ptr, workspace
 from .paged_attention import contiguous_layout, pool_layout
 
 
@@ -105,14 +105,17 @@ def _prepared_step(query, keys, values, summaries, *, top_blocks, local_window, 
     params = (query.shape, query.dtype, query.get_device(), top_blocks, local_window, block_size, superblock,
               top_super, float(router_scale), stream)
     key = (tuple(id(t) for t in held),) + params
-    hit = _STEP_CACHE.get(key)
+    # a captured step gets arguments and a workspace of its graph, and leaves nothing behind: only
+    # replays fill what it made
+    capturing = is_capturing()
+    hit = None if capturing else _STEP_CACHE.get(key)
     if hit is not None:
         entry, refs, ptrs = hit
         if all((r is None and t is None) or (r is not None and r() is t and t.data_ptr() == ptr)
                for r, t, ptr in zip(refs, held, ptrs)):
             return entry
     mkey = tuple(_meta(t) for t in held) + params
-    entry = _STEP_META.get(mkey)
+    entry = None if capturing else _STEP_META.get(mkey)
     if entry is not None:
         # same storage and metadata as a prepared form (a caller passing fresh views): the
         # identity key stays that of the tensors first prepared
@@ -132,9 +135,8 @@ def _prepared_step(query, keys, values, summaries, *, top_blocks, local_window, 
     borrowed = pr["summ"] is summaries and (super_summaries is None or sup is super_summaries) and (
         page_table is None or (pr["lens"] is context_lens and pr["layout"].page_table == page_table.data_ptr()
                                and page_table.dtype == torch.int32))
-    if not borrowed or torch.cuda.is_current_stream_capturing():
-        # converted copies: the arguments point into them, so the entry keeps them; what was made
-        # during a capture is that graph's own, and only its replays fill it
+    if not borrowed or capturing:
+        # converted copies: the arguments point into them, so the entry keeps them
         entry["keep"] = pr
         return entry
     _remember(_STEP_META, mkey, entry)

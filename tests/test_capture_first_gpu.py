@@ -65,3 +65,48 @@ def test_contiguous_decode_and_step():
     # bf16 probabilities and output: 2^-8 each of values below 6
     assert ((eager[0].double() - want).abs() <= 2 * 6 * 2.0 ** -8).all()
     assert spa.device_error_flags() == 0
+
+
+@pytest.mark.parametrize("what", ["decode", "step"])
+def test_graphs_replayed_side_by_side(what):
+    """Two graphs captured on one stream, after eager calls on it, give what they give alone while they
+    run at the same time on two streams, beside eager calls: their partial results lie apart."""
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    heads, dim, page, pages = 2, 128, 256, 64
+
+    def inputs():
+        k, v = (torch.randn(pages, heads, page, dim, generator=gen, device=DEV).bfloat16() for _ in range(2))
+        return (torch.randn(1, 8, dim, generator=gen, device=DEV).bfloat16(), k, v,
+                torch.randn(1, heads, pages, dim, generator=gen, device=DEV),
+                dict(page_table=torch.randperm(pages, generator=gen, device=DEV).int()[None],
+                     context_lens=torch.tensor([pages * page], dtype=torch.int32, device=DEV)))
+
+    def call(x):
+        q, k, v, summaries, more = x
+        if what == "decode":
+            return spa.paged_decode_attention(q, k, v, **more)
+        return spa.sparse_decode_step(q, k, v, summaries, top_blocks=24, local_window=page, block_size=page, **more)[0]
+
+    sets = [inputs() for _ in range(3)]
+    stream, streams, graphs = torch.cuda.Stream(), [torch.cuda.Stream() for _ in range(2)], []
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        want = [call(x).clone() for x in sets]
+    torch.cuda.synchronize()
+    for x in sets[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            out = [call(x) for _ in range(20)]
+        graphs.append((g, out))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(stream):
+            eager = [call(sets[2]) for _ in range(20)]
+        torch.cuda.synchronize()
+        for (_, outs), w in zip(graphs, want):
+            assert all(torch.equal(o, w) for o in outs)
+        assert all(torch.equal(o, want[2]) for o in eager)
+    assert spa.device_error_flags() == 0
