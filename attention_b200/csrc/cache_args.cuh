@@ -143,9 +143,9 @@ __device__ __forceinline__ void split_range(int n, int split, int nsplit, int& t
 
 // ---- Sharing out the work.  A pair is a (sequence, kv head, chunk of its query heads); all of a
 // sequence's pairs have its number of tiles.  The pairs' tiles, end to end, are cut into
-// sharing_ctas() equal ranges, one a CTA, however the lengths are spread; a range may end inside a pair, so a
-// pair's results are partials of consecutive CTAs, in slot CTA + pair (both only ever grow along
-// the ranges, so no two share a slot).  A pair that one CTA covers whole needs no partial.
+// sharing_ctas() equal ranges, one a CTA, however the lengths are spread; a range may end inside a
+// pair, so a pair's results are partials of consecutive CTAs, in slot CTA + pair (both only ever
+// grow along the ranges, so no two share a slot).  A pair that one CTA covers whole needs no partial.
 constexpr int kFlatBatch = 1024;  // longest batch whose prefix sums a CTA makes for itself
 
 // The launch has a.ctas CTAs, planned from the room that the contexts may grow into; where there

@@ -169,7 +169,8 @@ __global__ void __launch_bounds__(kFinishThreads) cache_decode_finish_kernel(con
     row = n % a.heads;
     first = last = pair;
     if (a.ctas)
-      ctas_of(before * pairs + static_cast<int64_t>(hc) * plan.n, plan.n, total * pairs, sharing_ctas(a, total * pairs), first, last);
+      ctas_of(before * pairs + static_cast<int64_t>(hc) * plan.n, plan.n, total * pairs,
+              sharing_ctas(a, total * pairs), first, last);
     first += pair, last += pair;
     if (first == last && !WEIGHTS) return 0.f;  // its CTA has written the output
     float M = -INFINITY;

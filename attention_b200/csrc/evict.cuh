@@ -336,8 +336,10 @@ __device__ __forceinline__ void compact_rows(U* pool, int rows, int per, int ran
         at.second();
         first(c + k + 4);
       }
+      __syncwarp();  // the cluster's barriers want whole warps
       cluster_arrive();
       if (c + k + 1 < chunks) load(c + k + 1, 1 - k);
+      __syncwarp();
       cluster_wait();
       if (c + k < chunks) store(c + k, k);
     }
